@@ -461,6 +461,71 @@ int ot_log_probs_given_den(const void *logits, int32_t dtype, const float *den,
                            int32_t targets_cols, int64_t rows, int32_t V,
                            int32_t blank, float *lp, void *stream);
 
+/* ---- answering with a joiner in 8 bits (no counterpart in the reference) ----
+ *
+ * Quantisation to e4m3 (OCP, largest value 448) with a float32 scale for each
+ * block of 128 elements of a row (block_rows = 1: activations) or of 128 rows
+ * (block_rows = 128: weights); last blocks may be partial:
+ *     scale  = max(fl32(max|x| / 448), 2^-126)
+ *     values = e4m3(fl32(x / scale))
+ * every rounding to nearest even, so the result is defined bit for bit.  A NaN
+ * or an infinity in a block makes its scale NaN or infinite.
+ *
+ * x (rows, D) of `dtype` (any of the three), element (r, d) at x[r * row_stride
+ * + d]; values (rows, D) bytes, row-major; scale (ceil(rows / block_rows),
+ * ceil(D / 128)).  rows = 0 does nothing. */
+int ot_quantize_blocks(const void *x, int32_t dtype, int64_t row_stride,
+                       int64_t rows, int32_t D, int32_t block_rows,
+                       void *values, float *scale, void *stream);
+
+/* ot_joiner_project for such operands:
+ *     logits[r, v] = bias[v] + sum_b x_scale[r, b] * weight_scale[v / 128, b]
+ *                              * sum_{k in block b} x[r, k] * weight[v, k]
+ * on the matrix cores with float32 accumulation, rounded once to logits_dtype
+ * (any of the three); den[r] = log sum_v exp(logits[r, v]) of the float32
+ * logits, before that rounding (den may be NULL).
+ *
+ * x (rows, D) and weight (V, D) e4m3 bytes, row-major, 16-byte aligned, D a
+ * multiple of 16; x_scale (rows, ceil(D / 128)), weight_scale (ceil(V / 128),
+ * ceil(D / 128)), bias (V) or NULL, float32.  With den the caller lends
+ * ot_joiner_project_blocks_workspace_bytes(rows, V) bytes, 8-byte aligned,
+ * contents irrelevant before and after.  rows = 0 does nothing. */
+size_t ot_joiner_project_blocks_workspace_bytes(int64_t rows, int32_t V);
+int ot_joiner_project_blocks(const void *x, const float *x_scale,
+                             const void *weight, const float *weight_scale,
+                             const float *bias, int64_t rows, int32_t D,
+                             int32_t V, void *logits, int32_t logits_dtype,
+                             float *den, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
+/* A symbol drawn from each row of logits by a given number uniform[r] of
+ * [0, 1).  With m the row's largest entry and T its temperature:
+ *     weights  w_i = exp((x_i - m) / T), 0 for x_i = -inf
+ *     order    larger values first, equal values by lower index
+ *     top_k    the first top_k entries of that order remain (<= 0: all)
+ *     top_p    of those, the entries in front of which the weights sum to less
+ *              than top_p times the sum of all of them (the first always;
+ *              >= 1: all)
+ *     min_p    of those, the entries with w_i >= min_p (<= 0: all; above 1: 1)
+ *     symbols[r]   = the first index, in index order, whose running sum of
+ *                    remaining weights exceeds uniform[r] times their total
+ *                    (uniform >= 1: the last one that remains)
+ *     log_probs[r] = log(w_symbol / total)
+ * T <= 0 or NaN: the first of the largest entries, log_probs 0.  A row without
+ * a largest finite entry (all -inf, a NaN, +inf) or with uniform NaN gives
+ * symbol -1 and log_probs -inf.  Weights and sums behave as in 64 bits.
+ *
+ * logits (rows, V) of `dtype` (any of the three), element (r, v) at
+ * logits[r * row_stride + v]; uniform, symbols, log_probs (rows).  Each setting
+ * is one value, or (pointer not NULL) one per row.  rows = 0 does nothing. */
+int ot_sample_symbols(const void *logits, int32_t dtype, int64_t row_stride,
+                      int64_t rows, int32_t V, const float *uniform,
+                      const float *temperature, float temperature_value,
+                      const int32_t *top_k, int32_t top_k_value,
+                      const float *top_p, float top_p_value,
+                      const float *min_p, float min_p_value, int32_t *symbols,
+                      float *log_probs, void *stream);
+
 /* Plain device-to-device copy kernel of n floats; used to calibrate profiler
  * byte counters against a transfer of known size. */
 int ot_copy_floats(const float *src, float *dst, int64_t n, void *stream);

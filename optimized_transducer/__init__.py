@@ -11,7 +11,8 @@ extension has not been built.
 # is not built)
 from .transducer_loss import TransducerLoss, TransducerLossFunction, transducer_loss  # noqa: F401,E402
 # what this build has beyond the reference, under the same roof
-from optimized_transducer_amd import joiner_transducer_loss, pack_joiner, project_joiner  # noqa: F401,E402
+from optimized_transducer_amd import (joiner_transducer_loss, pack_joiner, project_joiner,  # noqa: F401,E402
+                                      project_joiner_fp8, quantize_blocks, sample_symbols)
 
 __all__ = ["TransducerLoss", "transducer_loss", "pack_joiner", "project_joiner",
-           "joiner_transducer_loss"]
+           "joiner_transducer_loss", "quantize_blocks", "project_joiner_fp8", "sample_symbols"]

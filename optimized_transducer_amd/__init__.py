@@ -27,6 +27,7 @@ if _load_error is None:
     from .transducer_loss import TransducerLoss, TransducerLossFunction, transducer_loss  # noqa: E402,F401
     from .joiner import (PackJoinerFunction, ProjectJoinerFunction, joiner_transducer_loss,  # noqa: E402,F401
                          pack_joiner, project_joiner)
+    from .answering import project_joiner_fp8, quantize_blocks, sample_symbols  # noqa: E402,F401
 else:
     # Nothing works without the extension, and nothing pretends to: every name of the
     # package raises.  The import of the bare package itself succeeds so that
@@ -45,4 +46,5 @@ else:
         ) from _load_error
 
 __all__ = ["TransducerLoss", "TransducerLossFunction", "transducer_loss", "PackJoinerFunction",
-           "pack_joiner", "ProjectJoinerFunction", "project_joiner", "joiner_transducer_loss"]
+           "pack_joiner", "ProjectJoinerFunction", "project_joiner", "joiner_transducer_loss",
+           "quantize_blocks", "project_joiner_fp8", "sample_symbols"]

@@ -27,7 +27,7 @@ HIPCC_FLAGS = [
     "-ffp-contract=off", "-fno-fast-math", "-Wall",
 ]
 KERNEL_SOURCES = ("ot_kernels.hip", "ot_joiner.hip", "ot_half.hip", "ot_project.hip",
-                  "ot_project_grad.hip")
+                  "ot_project_grad.hip", "ot_quantize.hip", "ot_project_blocks.hip", "ot_sample.hip")
 OBJ_DIR = os.path.join(HERE, "build")  # objects only; ignored by git
 
 

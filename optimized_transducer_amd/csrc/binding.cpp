@@ -15,6 +15,7 @@
 #include <hip/hip_runtime_api.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdlib>
 #include <mutex>
@@ -837,6 +838,156 @@ std::pair<torch::Tensor, torch::Tensor> joiner_weight_grad(const torch::Tensor &
   return {grad_w, grad_b};
 }
 
+// ---- answering with a joiner in 8 bits ----
+
+int element_dtype(const torch::Tensor &t, const char *what) {
+  TORCH_CHECK(t.scalar_type() == torch::kFloat || t.scalar_type() == torch::kHalf ||
+                  t.scalar_type() == torch::kBFloat16,
+              what, " must be float32, float16 or bfloat16, got ", t.scalar_type());
+  return half_dtype(t);
+}
+
+// (rows, n) with unit column stride: any row pitch is read as it is
+torch::Tensor unit_columns(const torch::Tensor &t) {
+  return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous();
+}
+
+// e4m3 values of x (rows, D) in blocks of block_rows x 128 and their float32 scales
+// (ot_quantize_blocks).
+std::pair<torch::Tensor, torch::Tensor> quantize_blocks(const torch::Tensor &x_in, int64_t block_rows) {
+  const int dtype = element_dtype(x_in, "quantize_blocks: x");
+  TORCH_CHECK(x_in.is_cuda(), "quantize_blocks: x must be on a HIP device");
+  TORCH_CHECK(x_in.dim() == 2 && x_in.size(1) > 0 && x_in.size(0) <= INT32_MAX &&
+                  x_in.size(1) <= INT32_MAX - 128,
+              "quantize_blocks: x must have shape (rows, D) with D > 0, got ", x_in.sizes());
+  TORCH_CHECK(block_rows == 1 || block_rows == 128, "quantize_blocks: block_rows must be 1 or 128, got ",
+              block_rows);
+  const int64_t rows = x_in.size(0), D = x_in.size(1);
+  c10::hip::HIPGuardMasqueradingAsCUDA device_guard(x_in.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+  const torch::Tensor x = unit_columns(x_in);
+  torch::Tensor values = torch::empty({rows, D}, x.options().dtype(torch::kFloat8_e4m3fn));
+  torch::Tensor scale = torch::empty({(rows + block_rows - 1) / block_rows, (D + 127) / 128},
+                                     x.options().dtype(torch::kFloat));
+  ScopedTimer timer("quantize_blocks", stream);
+  OT_CHECK(ot_quantize_blocks(x.data_ptr(), dtype, x.stride(0), rows, (int32_t)D, (int32_t)block_rows,
+                              values.data_ptr(), scale.data_ptr<float>(), stream));
+  return {values, scale};
+}
+
+// Output projection of the joiner for such operands (ot_joiner_project_blocks): logits
+// (rows, V) of logits_dtype, and den (rows) or None.
+std::pair<torch::Tensor, torch::optional<torch::Tensor>> joiner_project_blocks(
+    const torch::Tensor &x, const torch::Tensor &x_scale, const torch::Tensor &weight,
+    const torch::Tensor &weight_scale, const torch::optional<torch::Tensor> &bias,
+    torch::ScalarType logits_dtype, bool denominators) {
+  TORCH_CHECK(x.scalar_type() == torch::kFloat8_e4m3fn && weight.scalar_type() == torch::kFloat8_e4m3fn,
+              "project_joiner_fp8: x and weight must be float8_e4m3fn, got ", x.scalar_type(), " and ",
+              weight.scalar_type());
+  TORCH_CHECK(x_scale.scalar_type() == torch::kFloat && weight_scale.scalar_type() == torch::kFloat,
+              "project_joiner_fp8: scales must be float32");
+  TORCH_CHECK(x.is_cuda() && weight.device() == x.device() && x_scale.device() == x.device() &&
+                  weight_scale.device() == x.device(),
+              "project_joiner_fp8: x, weight and their scales must be on one HIP device");
+  TORCH_CHECK(x.dim() == 2 && weight.dim() == 2 && x.size(1) == weight.size(1),
+              "project_joiner_fp8: expect x (rows, D) and weight (V, D), got ", x.sizes(), " and ",
+              weight.sizes());
+  const int64_t rows = x.size(0), D = x.size(1), V = weight.size(0), nb = (D + 127) / 128;
+  TORCH_CHECK(V > 0 && D > 0 && D % 16 == 0 && rows <= INT32_MAX && V <= INT32_MAX - 256 &&
+                  D <= INT32_MAX - 256,
+              "project_joiner_fp8 needs V > 0 and D a positive multiple of 16, got V = ", V, ", D = ", D);
+  TORCH_CHECK(x_scale.dim() == 2 && x_scale.size(0) == rows && x_scale.size(1) == nb,
+              "project_joiner_fp8: x_scale must have shape (rows, ceil(D / 128)), got ", x_scale.sizes());
+  TORCH_CHECK(weight_scale.dim() == 2 && weight_scale.size(0) == (V + 127) / 128 && weight_scale.size(1) == nb,
+              "project_joiner_fp8: weight_scale must have shape (ceil(V / 128), ceil(D / 128)), got ",
+              weight_scale.sizes());
+  TORCH_CHECK(x.is_contiguous() && weight.is_contiguous() && x_scale.is_contiguous() &&
+                  weight_scale.is_contiguous(),
+              "project_joiner_fp8: x, weight and their scales must be contiguous");
+  int out_dtype = OT_DTYPE_F32;
+  if (logits_dtype == torch::kHalf) out_dtype = OT_DTYPE_F16;
+  else if (logits_dtype == torch::kBFloat16) out_dtype = OT_DTYPE_BF16;
+  else TORCH_CHECK(logits_dtype == torch::kFloat,
+                   "project_joiner_fp8: logits_dtype must be float32, float16 or bfloat16, got ", logits_dtype);
+  c10::hip::HIPGuardMasqueradingAsCUDA device_guard(x.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+  torch::Tensor b;
+  if (bias.has_value() && bias->defined()) {
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == V && bias->device() == x.device(),
+                "project_joiner_fp8: bias must have shape (V,) on the device of x");
+    b = bias->detach().to(torch::kFloat).contiguous();
+  }
+  torch::Tensor logits = torch::empty({rows, V}, x.options().dtype(logits_dtype));
+  torch::Tensor den, workspace;
+  size_t ws_bytes = 0;
+  if (denominators) {
+    den = torch::empty({rows}, x.options().dtype(torch::kFloat));
+    ws_bytes = ot_joiner_project_blocks_workspace_bytes(rows, (int32_t)V);
+    workspace = torch::empty({(int64_t)ws_bytes}, x.options().dtype(torch::kUInt8));
+  }
+  ScopedTimer timer("joiner_project_blocks", stream);
+  OT_CHECK(ot_joiner_project_blocks(
+      x.data_ptr(), x_scale.data_ptr<float>(), weight.data_ptr(), weight_scale.data_ptr<float>(),
+      b.defined() ? b.data_ptr<float>() : nullptr, rows, (int32_t)D, (int32_t)V, logits.data_ptr(), out_dtype,
+      denominators ? den.data_ptr<float>() : nullptr, denominators ? workspace.data_ptr() : nullptr, ws_bytes,
+      stream));
+  return {logits, denominators ? torch::optional<torch::Tensor>(den) : torch::nullopt};
+}
+
+// A setting of sample_symbols given per row: (rows,) on the device of the logits.
+torch::Tensor row_setting(const torch::optional<torch::Tensor> &t, torch::ScalarType type,
+                          const torch::Tensor &logits, const char *name) {
+  if (!t.has_value() || !t->defined()) return torch::Tensor();
+  TORCH_CHECK(t->dim() == 1 && t->size(0) == logits.size(0) && t->device() == logits.device() &&
+                  t->scalar_type() == type,
+              "sample_symbols: ", name, " must be a number or a ", type,
+              " tensor of shape (rows,) on the device of logits");
+  return t->contiguous();
+}
+
+// A symbol drawn from each row of logits (ot_sample_symbols): (symbols int32, log_probs float32).
+std::pair<torch::Tensor, torch::Tensor> sample_symbols(
+    const torch::Tensor &logits_in, const torch::Tensor &uniform_in,
+    const torch::optional<torch::Tensor> &temperature, double temperature_value,
+    const torch::optional<torch::Tensor> &top_k, int64_t top_k_value,
+    const torch::optional<torch::Tensor> &top_p, double top_p_value,
+    const torch::optional<torch::Tensor> &min_p, double min_p_value) {
+  const int dtype = element_dtype(logits_in, "sample_symbols: logits");
+  TORCH_CHECK(logits_in.is_cuda(), "sample_symbols: logits must be on a HIP device");
+  TORCH_CHECK(logits_in.dim() == 2 && logits_in.size(1) > 0 && logits_in.size(0) <= INT32_MAX &&
+                  logits_in.size(1) <= INT32_MAX - 4096,
+              "sample_symbols: logits must have shape (rows, V) with V > 0, got ", logits_in.sizes());
+  const int64_t rows = logits_in.size(0), V = logits_in.size(1);
+  TORCH_CHECK(uniform_in.dim() == 1 && uniform_in.size(0) == rows && uniform_in.scalar_type() == torch::kFloat &&
+                  uniform_in.device() == logits_in.device(),
+              "sample_symbols: uniform must be a float32 tensor of shape (rows,) on the device of logits");
+  TORCH_CHECK(temperature.has_value() || temperature_value >= 0, "sample_symbols: temperature must be >= 0, got ",
+              temperature_value);
+  TORCH_CHECK(top_k.has_value() || top_k_value >= 0, "sample_symbols: top_k must be >= 0, got ", top_k_value);
+  TORCH_CHECK(top_p.has_value() || (top_p_value >= 0 && top_p_value <= 1),
+              "sample_symbols: top_p must be in [0, 1], got ", top_p_value);
+  TORCH_CHECK(min_p.has_value() || (min_p_value >= 0 && min_p_value <= 1),
+              "sample_symbols: min_p must be in [0, 1], got ", min_p_value);
+  c10::hip::HIPGuardMasqueradingAsCUDA device_guard(logits_in.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+  const torch::Tensor logits = unit_columns(logits_in), uniform = uniform_in.contiguous();
+  const torch::Tensor t = row_setting(temperature, torch::kFloat, logits, "temperature");
+  const torch::Tensor k = row_setting(top_k, torch::kInt32, logits, "top_k");
+  const torch::Tensor p = row_setting(top_p, torch::kFloat, logits, "top_p");
+  const torch::Tensor q = row_setting(min_p, torch::kFloat, logits, "min_p");
+  torch::Tensor symbols = torch::empty({rows}, logits.options().dtype(torch::kInt32));
+  torch::Tensor log_probs = torch::empty({rows}, logits.options().dtype(torch::kFloat));
+  ScopedTimer timer("sample_symbols", stream);
+  OT_CHECK(ot_sample_symbols(
+      logits.data_ptr(), dtype, logits.stride(0), rows, (int32_t)V, uniform.data_ptr<float>(),
+      t.defined() ? t.data_ptr<float>() : nullptr, (float)temperature_value,
+      k.defined() ? k.data_ptr<int32_t>() : nullptr, (int32_t)std::min<int64_t>(top_k_value, INT32_MAX),
+      p.defined() ? p.data_ptr<float>() : nullptr, (float)top_p_value,
+      q.defined() ? q.data_ptr<float>() : nullptr, (float)min_p_value, symbols.data_ptr<int32_t>(),
+      log_probs.data_ptr<float>(), stream));
+  return {symbols, log_probs};
+}
+
 PYBIND11_MODULE(_optimized_transducer, m) {
   m.doc() = "MI355X-native transducer loss (drop-in for optimized_transducer's extension module)";
 #ifdef OT_BUILT_WITH_TORCH
@@ -896,6 +1047,19 @@ PYBIND11_MODULE(_optimized_transducer, m) {
   m.def("joiner_weight_grad", &joiner_weight_grad, py::arg("grad_logits"), py::arg("x"),
         "Backward of joiner_project in its parameters: (grad_logits.T @ x in x's dtype, "
         "grad_logits.sum(0) in float32) for float16 / bfloat16 operands, float32 accumulation.");
+  m.def("quantize_blocks", &quantize_blocks, py::arg("x"), py::arg("block_rows"));
+  m.def("joiner_project_blocks",
+        [](const torch::Tensor &x, const torch::Tensor &x_scale, const torch::Tensor &weight,
+           const torch::Tensor &weight_scale, const torch::optional<torch::Tensor> &bias,
+           py::object logits_dtype, bool denominators) {
+          return joiner_project_blocks(x, x_scale, weight, weight_scale, bias,
+                                       torch::python::detail::py_object_to_dtype(logits_dtype), denominators);
+        },
+        py::arg("x"), py::arg("x_scale"), py::arg("weight"), py::arg("weight_scale"), py::arg("bias"),
+        py::arg("logits_dtype"), py::arg("denominators"));
+  m.def("sample_symbols", &sample_symbols, py::arg("logits"), py::arg("uniform"), py::arg("temperature"),
+        py::arg("temperature_value"), py::arg("top_k"), py::arg("top_k_value"), py::arg("top_p"),
+        py::arg("top_p_value"), py::arg("min_p"), py::arg("min_p_value"));
   m.def("set_profiling", &set_profiling, py::arg("on"));
   m.def("set_overlap", &set_overlap, py::arg("on"),
         "Run the lattice kernel of one half of a large batch on a second stream while the "
