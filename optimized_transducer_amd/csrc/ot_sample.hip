@@ -12,8 +12,24 @@
 // T = 0: the first of the largest entries, log_prob 0.  A row with no largest finite entry
 // (all -inf, a NaN, +inf) has symbol -1, log_prob -inf; so has u = NaN.
 //
-// Which index a symbol falls on hangs on the last bits of a running sum, so weights and sums
-// are held in 64 bits.
+// Which index a symbol falls on, or where top_p cuts, hangs on the last bits of a sum, and the
+// answer is that of 64-bit weights and sums.  It is first looked for with 32-bit weights and a
+// bound on how far off their sums can be: only a row where a decision lies inside the bound
+// (about 4 * V * kUnit rows of one, 0.2 % at V = 500) is done again in 64 bits.
+//
+// The bound.  A 32-bit weight is off by a relative 2^-24 * |z| (the rounding of x - m, z the
+// exponent), 2^-23 (the hardware's 2^x) and 2^-24 (a last rounding); a sum of 8 adds 3 * 2^-24,
+// all longer sums are 64-bit.  Weighted with w, the |z| of a set that holds the largest entry
+// average to its entropy minus the logarithm of its total, so to ln V at most.  Any partial sum
+// is off by less than (ln V + 8) * 2^-24 of the set's total, and so is u or top_p times it.
+//
+// No sort: a cut is found by a histogram of the interval that still holds it, 256 bins at a
+// time, until one value is left; two levels do for rows without many equal values.
+//
+// A row is worked on by one wave (short rows: its elements stay in registers, four rows per
+// workgroup and no barrier), by 4 or 16 waves with the elements in registers, or by 16 waves
+// that read it again in each step (long rows, served by the caches).  Every wave owns a
+// contiguous part of the row, so that a running sum needs one number from each wave.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -30,222 +46,772 @@ struct SampleSettings {
   int32_t top_k_value;
 };
 
+constexpr int kSampleBins = 256;
+constexpr float kUnit = 5.9604644775390625e-08f;  // 2^-24
+constexpr float kInf = __builtin_huge_valf();
+
+// ---- wave-wide helpers ----------------------------------------------------------------------
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or_zero(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_or_zero(double v) {
+  const int64_t b = __builtin_bit_cast(int64_t, v);
+  const unsigned lo = (unsigned)dpp_or_zero<CTRL, ROWS>((int)b);
+  const unsigned hi = (unsigned)dpp_or_zero<CTRL, ROWS>((int)(b >> 32));
+  return __builtin_bit_cast(double, (int64_t)lo | ((int64_t)hi << 32));
+}
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ float lane_value(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+__device__ __forceinline__ double lane_value(double v, int lane) {
+  const int64_t b = __builtin_bit_cast(int64_t, v);
+  const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)b, lane);
+  const unsigned hi = (unsigned)__builtin_amdgcn_readlane((int)(b >> 32), lane);
+  return __builtin_bit_cast(double, (int64_t)lo | ((int64_t)hi << 32));
+}
+
+// sum over the lanes up to and including this one: inside rows of 16 lanes (row_shr), then the
+// last lane of a row to the next one (row_bcast)
+template <class N>
+__device__ __forceinline__ N wave_scan(N v) {
+  v += dpp_or_zero<0x111, 0xf>(v);
+  v += dpp_or_zero<0x112, 0xf>(v);
+  v += dpp_or_zero<0x114, 0xf>(v);
+  v += dpp_or_zero<0x118, 0xf>(v);
+  v += dpp_or_zero<0x142, 0xa>(v);
+  v += dpp_or_zero<0x143, 0xc>(v);
+  return v;
+}
+__device__ __forceinline__ double wave_sum(double v) { return lane_value(wave_scan(v), kWave - 1); }
+__device__ __forceinline__ int wave_sum(int v) { return lane_value(wave_scan(v), kWave - 1); }
+
+// ---- the threads that share a row -----------------------------------------------------------
+
+template <int WAVES>
+struct SampleShared {
+  double bin_weight[kSampleBins];
+  unsigned bin_count[kSampleBins];
+  double sum[WAVES];
+  float value[2][WAVES];
+  int count[WAVES];
+  int index;
+};
+
+template <int WAVES>
+struct RowGroup {
+  SampleShared<WAVES> &s;
+  int lane, wave;
+
+  __device__ __forceinline__ int thread() const { return wave * kWave + lane; }
+  __device__ __forceinline__ void sync() const {
+    if constexpr (WAVES == 1) {
+      // one wave: LDS operations of a wave run in order
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    } else {
+      __syncthreads();
+    }
+  }
+  // the largest hi and the smallest lo
+  __device__ __forceinline__ void extremes(float &hi, float &lo) const {
+    hi = group_allreduce<kWave>(hi, MaxOp());
+    lo = -group_allreduce<kWave>(-lo, MaxOp());
+    if constexpr (WAVES > 1) {
+      sync();
+      if (lane == 0) {
+        s.value[0][wave] = hi;
+        s.value[1][wave] = lo;
+      }
+      sync();
+#pragma unroll
+      for (int k = 0; k < WAVES; ++k) {
+        hi = fmaxf(hi, s.value[0][k]);
+        lo = fminf(lo, s.value[1][k]);
+      }
+    }
+  }
+  // totals of a sum and a count, the same bits in every thread
+  __device__ __forceinline__ void totals(double &sum, int &count) const {
+    sum = wave_sum(sum);
+    count = wave_sum(count);
+    if constexpr (WAVES > 1) {
+      sync();
+      if (lane == 0) {
+        s.sum[wave] = sum;
+        s.count[wave] = count;
+      }
+      sync();
+      sum = 0.0;
+      count = 0;
+#pragma unroll
+      for (int k = 0; k < WAVES; ++k) {
+        sum += s.sum[k];
+        count += s.count[k];
+      }
+    }
+  }
+};
+
+// elements per 16-byte load
+template <class T> constexpr int kSampleVec = sizeof(T) == 4 ? 4 : 8;
+
+// elements [i, i + VEC) of a row of V; those past the end are -inf
+template <class T>
+__device__ __forceinline__ void load_logits(const void *row, int i, int V, float x[]) {
+  constexpr int VEC = kSampleVec<T>;
+  if (i + VEC <= V) {
+    // the row may start anywhere its type can
+    if constexpr (VEC == 4) {
+      typedef f32x4 unaligned __attribute__((aligned(4)));
+      const f32x4 v = *reinterpret_cast<const unaligned *>(static_cast<const float *>(row) + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = v[e];
+    } else {
+      typedef u32x4 unaligned __attribute__((aligned(2)));
+      const u32x4 v = *reinterpret_cast<const unaligned *>(static_cast<const unsigned short *>(row) + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const unsigned w = v[e];
+        x[2 * e] = to_float<T>((unsigned short)(w & 0xffffu));
+        x[2 * e + 1] = to_float<T>((unsigned short)(w >> 16));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) x[e] = i + e < V ? load_element<T>(row, i + e) : OT_NEG_INF;
+  }
+}
+
+// exp((x - m) / T) in 32 bits for m < 1e30 and T of [1e-30, 1e30]; c_hi + c_lo = log2(e) / T.
+// 2^(d * c) as the product's rounded part through the hardware unit and its residual to first
+// order, so that the argument's error does not grow with it.
+struct FastWeight {
+  float m, c_hi, c_lo, d_min;
+  FastWeight() = default;
+  __device__ __forceinline__ FastWeight(float m_, float T) : m(m_) {
+    constexpr float kLog2eHi = 1.44269502162933349609375f, kLog2eLo = 1.92596299112661746e-8f;
+    const float r = 1.0f / T, e = __builtin_fmaf(-T, r, 1.0f);  // 1 / T = r + r * e + ...
+    c_hi = r * kLog2eHi;
+    c_lo = __builtin_fmaf(r, kLog2eHi, -c_hi) + __builtin_fmaf(r * e, kLog2eHi, r * kLog2eLo);
+    d_min = -160.f / c_hi;  // 2^-160 is 0, and the residual of -inf would be a NaN
+  }
+  __device__ __forceinline__ float operator()(float x) const {
+    constexpr float kLn2 = 0.693147182464599609375f;
+    const float d = fmaxf(x - m, d_min);
+    const float ph = d * c_hi;
+    const float pl = __builtin_fmaf(d, c_lo, __builtin_fmaf(d, c_hi, -ph));
+    const float e = __builtin_amdgcn_exp2f(ph);
+    return __builtin_fmaf(e, pl * kLn2, e);
+  }
+};
+// the same in 64 bits, for any m and T > 0
+struct FullWeight {
+  double m, T;
+  FullWeight() = default;
+  __device__ __forceinline__ FullWeight(float m_, float T_) : m(m_), T(T_) {}
+  __device__ __forceinline__ double operator()(float x) const {
+    return x == OT_NEG_INF ? 0.0 : exp(((double)x - m) / T);
+  }
+};
+
 // unsigned integers that order like the values (both zeros alike)
 __device__ __forceinline__ unsigned order_key(float x) {
   const unsigned b = __builtin_bit_cast(unsigned, x + 0.0f);
   return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-template <class V, class Op>
-__device__ __forceinline__ V block_reduce(V v, Op op, V *s) {
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) v = op(v, __shfl_xor(v, d, kWave));
-  __syncthreads();  // the previous use of s has been read
-  if (threadIdx.x % kWave == 0) s[threadIdx.x / kWave] = v;
-  __syncthreads();
-  v = s[0];
-#pragma unroll
-  for (int k = 1; k < kWavesPerBlock; ++k) v = op(v, s[k]);
-  return v;
-}
+// one row's answer
+struct Drawn {
+  int symbol;
+  float log_prob;
+  bool sure;
+};
 
-// sum of v over the threads up to and including this one; *total: over all
-template <class V>
-__device__ __forceinline__ V block_scan(V v, V *s, V *total) {
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const V up = __shfl_up(v, d, kWave);
-    if (lane >= d) v += up;
+// Draws from a row with a finite largest entry m at a temperature above 0.  Every thread of the
+// group calls it with the same arguments and gets the same answer.
+//   CHUNKS > 0: wave w holds elements [w * CHUNKS * 64 * VEC, + CHUNKS * 64 * VEC) in x, chunk by
+//     chunk, lane by lane (VEC consecutive ones each); excluded entries become -inf there
+//   CHUNKS = 0: the row is read from memory in every step; `per_wave` chunks per wave
+//   Weight: FastWeight (32 bits, with `bound` > 0) or FullWeight (64 bits)
+template <class T, int WAVES, int CHUNKS, class Weight>
+struct Sampler {
+  static constexpr int VEC = kSampleVec<T>;
+  static constexpr bool kHeld = CHUNKS > 0;
+  static constexpr bool kFast = __is_same(Weight, FastWeight);
+  typedef decltype(Weight()(0.f)) W;
+
+  const RowGroup<WAVES> &g;
+  const void *row;
+  const int V, per_wave;
+  const float m, T_;
+  const Weight weight;
+  const double bound;
+  float (&x)[kHeld ? CHUNKS : 1][VEC];
+  bool sure = true;
+  W w[kHeld ? CHUNKS : 1][VEC];
+  // not held: entries below `floor_`, and those at it behind index `floor_last`, are excluded;
+  // so are weights below least
+  float floor_ = OT_NEG_INF;
+  int floor_last = 0x7fffffff;
+  W least = 0;
+
+  __device__ __forceinline__ Sampler(const RowGroup<WAVES> &g_, const void *row_, int V_, int per_wave_, float m_,
+                                     float temperature, double bound_, float (&x_)[kHeld ? CHUNKS : 1][VEC])
+      : g(g_), row(row_), V(V_), per_wave(per_wave_), m(m_), T_(temperature), weight(m_, temperature),
+        bound(bound_), x(x_) {}
+
+  __device__ __forceinline__ int chunks() const { return kHeld ? CHUNKS : per_wave; }
+  __device__ __forceinline__ int first_index(int j) const {
+    return ((g.wave * chunks() + j) * kWave + g.lane) * VEC;
   }
-  __syncthreads();
-  if (lane == kWave - 1) s[wave] = v;
-  __syncthreads();
-  V before = 0, all = 0;
+  // f(j, i, x of the chunk) for each chunk of this lane, i the index of its first element
+  template <class F>
+  __device__ __forceinline__ void each(F f) {
+    if constexpr (kHeld) {
 #pragma unroll
-  for (int k = 0; k < kWavesPerBlock; ++k) {
-    if (k < wave) before += s[k];
-    all += s[k];
+      for (int j = 0; j < CHUNKS; ++j) f(j, first_index(j), x[j]);
+    } else {
+      for (int j = 0; j < per_wave; ++j) {
+        const int i = first_index(j);
+        float y[VEC];
+        load_logits<T>(row, i, V, y);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (y[e] < floor_ || (y[e] == floor_ && i + e > floor_last)) y[e] = OT_NEG_INF;
+        f(j, i, y);
+      }
+    }
   }
-  *total = all;
-  return before + v;
-}
+  __device__ __forceinline__ W weight_of(int j, int e, float y) {
+    if constexpr (kHeld) return w[j][e];
+    const W v = weight(y);
+    return v >= least ? v : (W)0;
+  }
+  // sum of a chunk's VEC weights, pairwise
+  __device__ __forceinline__ static W pairwise(const W v[VEC]) {
+    if constexpr (VEC == 4) return (v[0] + v[1]) + (v[2] + v[3]);
+    else return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+  }
 
-// A workgroup per row; every step reads the row again.
-template <class T>
-__global__ __launch_bounds__(kBlock) void sample_row_kernel(const void *__restrict__ logits, int64_t row_stride,
-                                                            int64_t rows, int V,
-                                                            const float *__restrict__ uniform,
-                                                            SampleSettings set, int32_t *__restrict__ symbols,
-                                                            float *__restrict__ log_probs) {
-  __shared__ unsigned s_u[kWavesPerBlock];
-  __shared__ int s_i[kWavesPerBlock];
-  __shared__ double s_d[kWavesPerBlock];
-  auto max_u = [](unsigned a, unsigned b) { return max(a, b); };
-  auto min_i = [](int a, int b) { return min(a, b); };
-  auto sum_i = [](int a, int b) { return a + b; };
-  auto sum_d = [](double a, double b) { return a + b; };
-  const int tid = threadIdx.x;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int64_t base = row * row_stride;
-    const float temperature = set.temperature ? set.temperature[row] : set.temperature_value;
-    const float top_p = set.top_p ? set.top_p[row] : set.top_p_value;
-    const float min_p_row = set.min_p ? set.min_p[row] : set.min_p_value;
-    const double min_p = min_p_row > 0.f ? fminf(min_p_row, 1.f) : 0.f;
-    const int top_k = set.top_k ? set.top_k[row] : set.top_k_value;
-    const double u = uniform[row];
-    auto at = [&](int i) { return load_element<T>(logits, base + i); };
+  // Excludes the entries below v, and those at v behind the first n.
+  __device__ __forceinline__ void exclude(float v, int n, int at_v) {
+    int last = 0x7fffffff;
+    if (n < at_v) {  // the index of entry number n of those at v
+      int mine = 0;
+      each([&](int, int, const float *y) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) mine += y[e] == v;
+      });
+      const int here = wave_sum(mine);
+      int before = 0;
+      g.sync();
+      if constexpr (WAVES > 1) {
+        if (g.lane == 0) g.s.count[g.wave] = here;
+      }
+      if (g.thread() == 0) g.s.index = -1;
+      g.sync();
+      if constexpr (WAVES > 1) {
+        for (int k = 0; k < g.wave; ++k) before += g.s.count[k];
+      }
+      if (before < n && n <= before + here) {
+        each([&](int, int i, const float *y) {
+          int c = 0;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) c += y[e] == v;
+          const int upto = wave_scan(c);
+          int seen = before + upto - c;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            seen += y[e] == v;
+            if (y[e] == v && seen == n) g.s.index = i + e;
+          }
+          before += lane_value(upto, kWave - 1);
+        });
+      }
+      g.sync();
+      last = g.s.index;
+    }
+    if constexpr (kHeld) {
+#pragma unroll
+      for (int j = 0; j < CHUNKS; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (x[j][e] < v || (x[j][e] == v && first_index(j) + e > last)) {
+            x[j][e] = OT_NEG_INF;
+            w[j][e] = 0;
+          }
+    } else {
+      floor_last = v == floor_ ? min(last, floor_last) : last;
+      floor_ = v;
+    }
+  }
 
-    // largest entry; a NaN outranks everything
-    unsigned key = 0;
-    for (int i = tid; i < V; i += kBlock) {
-      const float x = at(i);
-      key = max(key, x != x ? 0xffffffffu : order_key(x));
-    }
-    const unsigned top_key = block_reduce(key, max_u, s_u);
-    constexpr unsigned kNegInfKey = 0x007fffffu, kPosInfKey = 0xff800000u;
-    if (top_key <= kNegInfKey || top_key >= kPosInfKey || u != u) {
-      if (tid == 0) {
-        symbols[row] = -1;
-        log_probs[row] = OT_NEG_INF;
+  // The largest value v such that the entries at or above it (their number, or with WEIGHTS
+  // their weights) reach `want`; by_above: what the entries above v come to.  With weights this
+  // goes by sums in whatever order the bins were filled: close, and for the caller to check.
+  template <bool WEIGHTS>
+  __device__ __forceinline__ float select(double want, float lo, double &above) {
+    float hi = m;
+    above = 0.0;
+    while (lo < hi) {
+      for (int i = g.thread(); i < kSampleBins; i += WAVES * kWave) {
+        g.s.bin_count[i] = 0;
+        if (WEIGHTS) g.s.bin_weight[i] = 0.0;
       }
-      continue;
-    }
-    if (!(temperature > 0.f)) {
-      int first = V;
-      for (int i = tid; i < V; i += kBlock)
-        if (first == V && order_key(at(i)) == top_key) first = i;
-      first = block_reduce(first, min_i, s_i);
-      if (tid == 0) {
-        symbols[row] = first;
-        log_probs[row] = 0.f;
+      g.sync();
+      // bins of equal width; where that is no normal number, bins of the values' bit patterns.
+      // Either way hi falls into the first bin and lo into the last.
+      const float half = 0.5f * hi - 0.5f * lo;
+      const bool by_value = half > 1e-30f;
+      const float per_unit = by_value ? (0.5f * kSampleBins) / half : 0.f;
+      const unsigned hi_key = order_key(hi);
+      const int shift = max(0, 24 - __clz(hi_key - order_key(lo)));
+      auto bin = [&](float y) -> int {
+        return by_value ? (int)fminf((hi - y) * per_unit, kSampleBins - 1.0f)
+                        : (int)((hi_key - order_key(y)) >> shift);
+      };
+      each([&](int j, int, const float *y) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (y[e] >= lo && y[e] <= hi) {
+            const int b = bin(y[e]);
+            atomicAdd(&g.s.bin_count[b], 1u);
+            if (WEIGHTS) {
+              if constexpr (kFast)
+                unsafeAtomicAdd(reinterpret_cast<float *>(g.s.bin_weight) + b, (float)weight_of(j, e, y[e]));
+              else
+                unsafeAtomicAdd(&g.s.bin_weight[b], (double)weight_of(j, e, y[e]));
+            }
+          }
+      });
+      g.sync();
+      // every wave looks for the bin: lane l holds bins [4 l, 4 l + 4)
+      constexpr int kPer = kSampleBins / kWave;
+      unsigned n[kPer];
+      double amount[kPer], mine = 0.0;
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        const int b = g.lane * kPer + q;
+        n[q] = g.s.bin_count[b];
+        amount[q] = !WEIGHTS ? (double)n[q]
+                    : kFast  ? (double)reinterpret_cast<const float *>(g.s.bin_weight)[b]
+                             : g.s.bin_weight[b];
+        mine += amount[q];
       }
-      continue;
-    }
-    const double m = __builtin_bit_cast(float, top_key ^ ((top_key >> 31) ? 0x80000000u : 0xffffffffu));
-    const double T_ = temperature;
-    auto weight = [&](float x) { return x == OT_NEG_INF ? 0.0 : exp(((double)x - m) / T_); };
-
-    // Remaining entries: those with a key above `cut`, and the first `ties` of those at it.
-    unsigned cut = 0;
-    int ties = V;
-    if (top_k > 0 && top_k < V) {
-      // the largest key that top_k entries reach, bit by bit
-      unsigned k = 0;
-      for (int bit = 31; bit >= 0; --bit) {
-        const unsigned t = k | (1u << bit);
-        int n = 0;
-        for (int i = tid; i < V; i += kBlock) n += order_key(at(i)) >= t;
-        if (block_reduce(n, sum_i, s_i) >= top_k) k = t;
-      }
-      int above = 0;
-      for (int i = tid; i < V; i += kBlock) above += order_key(at(i)) > k;
-      cut = k;
-      ties = top_k - block_reduce(above, sum_i, s_i);
-    }
-    if (top_p < 1.f) {
-      const double w_cut = weight(__builtin_bit_cast(float, cut ^ ((cut >> 31) ? 0x80000000u : 0xffffffffu)));
-      double sum = 0.0;
-      int at_cut = 0;
-      for (int i = tid; i < V; i += kBlock) {
-        const float x = at(i);
-        const unsigned q = order_key(x);
-        if (q > cut) sum += weight(x);
-        at_cut += q == cut;
-      }
-      const int limit = min(ties, block_reduce(at_cut, sum_i, s_i));
-      const double above_cut = block_reduce(sum, sum_d, s_d);
-      const double want = (double)top_p * (above_cut + (limit > 0 ? limit * w_cut : 0.0));
-      // the largest key above `cut` whose entries and those above reach `want`; none: `cut`
-      unsigned k = 0;
-      for (int bit = 31; bit >= 0; --bit) {
-        const unsigned t = k | (1u << bit);
-        if (t <= cut) {
-          k = t;  // all of them reach it
-          continue;
-        }
-        sum = 0.0;
-        for (int i = tid; i < V; i += kBlock) {
-          const float x = at(i);
-          if (order_key(x) >= t) sum += weight(x);
-        }
-        if (block_reduce(sum, sum_d, s_d) >= want && t <= top_key) k = t;
-      }
-      if (k < cut) k = cut;
-      const float xk = __builtin_bit_cast(float, k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
-      const double wk = weight(xk);
-      sum = 0.0;
-      at_cut = 0;
-      for (int i = tid; i < V; i += kBlock) {
-        const float x = at(i);
-        const unsigned q = order_key(x);
-        if (q > k) sum += weight(x);
-        at_cut += q == k;
-      }
-      at_cut = block_reduce(at_cut, sum_i, s_i);
-      sum = block_reduce(sum, sum_d, s_d);
-      if (k == cut) at_cut = min(at_cut, ties);
-      // entry number j of the ties remains if sum + j * wk < want
-      int n = at_cut;
-      if (wk > 0.0) {
-        const double q = ceil((want - sum) / wk);
-        n = q < 1.0 ? 0 : q < at_cut ? (int)q : at_cut;
-      }
-      if (k == top_key) n = max(n, 1);
-      cut = k;
-      ties = n;
-    }
-
-    // total of the remaining weights, then the index where the running sum passes u times it.
-    // Thread t holds entry t of a run of 256; ties count along the way.
-    double total = 0.0, target = 0.0;
-    int symbol = -1, last = -1;
-    for (int pass = 0; pass < 2; ++pass) {
-      double run = 0.0;
-      int seen = 0;
-      for (int i0 = 0; i0 < V; i0 += kBlock) {
-        const int i = i0 + tid;
-        float x = i < V ? at(i) : OT_NEG_INF;
-        const unsigned q = order_key(x);
-        int tie_total;
-        const int tie = block_scan(i < V && q == cut ? 1 : 0, s_i, &tie_total);
-        const bool remains = i < V && (q > cut || (q == cut && seen + tie <= ties));
-        double w = remains ? weight(x) : 0.0;
-        if (!(w >= min_p)) w = 0.0;
-        seen += tie_total;
-        double sum;
-        const double upto = run + block_scan(w, s_d, &sum);
-        if (pass == 1) {
-          const int hit = block_reduce(upto > target && w > 0.0 ? i : V, min_i, s_i);
-          const int any = block_reduce(w > 0.0 ? i : -1, [](int a, int b) { return max(a, b); }, s_i);
-          if (any >= 0) last = any;
-          if (hit < V) {
-            symbol = hit;
-            break;
+      double run = above + (wave_scan(mine) - mine);
+      int reached = kSampleBins, filled = -1;
+      double before_reached = 0.0, before_filled = 0.0;
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        if (n[q] > 0) {
+          filled = g.lane * kPer + q;
+          before_filled = run;
+          if (reached == kSampleBins && run + amount[q] >= want) {
+            reached = filled;
+            before_reached = run;
           }
         }
-        run += sum;
+        run += amount[q];
       }
-      if (pass == 0) {
-        total = run;
-        target = u * total;
-      }
+      const uint64_t r = __ballot(reached < kSampleBins), f = __ballot(filled >= 0);
+      // (rounding alone can keep the last bin from reaching `want`)
+      const int src = r ? __builtin_ctzll(r) : 63 - __builtin_clzll(f);
+      const int pick = r ? lane_value(reached, src) : lane_value(filled, src);
+      above = r ? lane_value(before_reached, src) : lane_value(before_filled, src);
+      float b_hi = OT_NEG_INF, b_lo = kInf;
+      each([&](int, int, const float *y) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (y[e] >= lo && y[e] <= hi && bin(y[e]) == pick) {
+            b_hi = fmaxf(b_hi, y[e]);
+            b_lo = fminf(b_lo, y[e]);
+          }
+      });
+      g.sync();  // the bins have been read
+      g.extremes(b_hi, b_lo);
+      hi = b_hi;
+      lo = b_lo;
     }
-    if (symbol < 0) symbol = last;  // u >= 1, or a sum that rounds to it
-    if (tid == 0) {
-      symbols[row] = symbol;
-      log_probs[row] = (float)(((double)at(symbol) - m) / T_ - log(total));
+    return lo;
+  }
+
+  // the smallest entry that is not excluded
+  __device__ __forceinline__ float smallest() {
+    float hi = OT_NEG_INF, lo = kInf;
+    each([&](int, int, const float *y) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (y[e] > OT_NEG_INF) lo = fminf(lo, y[e]);
+    });
+    g.extremes(hi, lo);
+    return lo;
+  }
+
+  __device__ __forceinline__ void keep_top_k(int k) {
+    const float lo = smallest();
+    double finite = 0.0;
+    int count = 0;
+    each([&](int, int, const float *y) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) count += y[e] > OT_NEG_INF;
+    });
+    g.totals(finite, count);
+    if (k >= count) return;
+    double above;
+    const float v = select<false>((double)k, lo, above);
+    int at_v = 0;
+    each([&](int, int, const float *y) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) at_v += y[e] == v;
+    });
+    double none = 0.0;
+    g.totals(none, at_v);
+    exclude(v, k - (int)above, at_v);
+  }
+
+  // sum of the weights above v, and the number of entries at it
+  __device__ __forceinline__ void sum_above(float v, double &sum, int &at_v) {
+    sum = 0.0;
+    at_v = 0;
+    each([&](int j, int, const float *y) {
+      W t[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        t[e] = y[e] > v ? weight_of(j, e, y[e]) : (W)0;
+        at_v += y[e] == v;
+      }
+      sum += (double)pairwise(t);
+    });
+    g.totals(sum, at_v);
+  }
+
+  __device__ __forceinline__ void keep_top_p(float p) {
+    double total;
+    int none;
+    sum_above(OT_NEG_INF, total, none);
+    const double want = (double)p * total;
+    double above, sum;
+    const float v = select<true>(want, smallest(), above);
+    int at_v;
+    sum_above(v, sum, at_v);
+    const double wv = (double)weight(v);
+    // of the entries at v, number j (from 0) remains if sum + j * wv < want
+    int n = at_v;
+    if (wv > 0.0) {
+      const double q = ceil((want - sum) / wv);
+      n = q < 1.0 ? 0 : q < at_v ? (int)q : at_v;
+    }
+    if (v == m) n = max(n, 1);
+    if (kFast) {
+      const double off = 2.0 * bound * total;
+      const bool first = v == m && n == 1;  // remains whatever `want` is
+      if (!(first || (n >= 1 && sum + (n - 1) * wv < want - off)) || !(sum + n * wv >= want + off)) sure = false;
+    }
+    exclude(v, n, at_v);
+  }
+
+  __device__ __forceinline__ void keep_min_p(float p) {
+    if constexpr (kHeld) {
+      bool near = false;
+#pragma unroll
+      for (int j = 0; j < CHUNKS; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          // a 32-bit weight is within 2^-24 * (|z| + 3) of the 64-bit one, |z| < 104 here
+          if (kFast && x[j][e] < m && __builtin_fabsf((float)w[j][e] - p) <= 128.f * kUnit * p) near = true;
+          if (!(w[j][e] >= (W)p)) w[j][e] = 0;
+        }
+      if (kFast && any(near)) sure = false;
+    } else {
+      least = (W)p;
+      if constexpr (kFast) {
+        bool near = false;
+        each([&](int, int, const float *y) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (y[e] < m && __builtin_fabsf((float)weight(y[e]) - p) <= 128.f * kUnit * p) near = true;
+        });
+        if (any(near)) sure = false;
+      }
     }
   }
+  __device__ __forceinline__ bool any(bool b) {
+    float hi = b ? 1.f : 0.f, lo = 0.f;
+    g.extremes(hi, lo);
+    return hi > 0.f;
+  }
+
+  __device__ __forceinline__ Drawn draw(double u, int top_k, float top_p, float min_p) {
+    if (top_k > 0 && top_k < V) keep_top_k(top_k);
+    if constexpr (kHeld) {
+#pragma unroll
+      for (int j = 0; j < CHUNKS; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[j][e] = weight(x[j][e]);
+    }
+    if (top_p < 1.f) keep_top_p(top_p);
+    if (kFast && !sure) return {0, 0.f, false};
+    if (min_p > 0.f) keep_min_p(fminf(min_p, 1.f));
+    if (kFast && !sure) return {0, 0.f, false};
+
+    // totals of the waves' parts, then the part, the chunk, the lane and the element in which
+    // the running sum passes u * total
+    double part = 0.0;
+    each([&](int j, int, const float *y) {
+      W t[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) t[e] = weight_of(j, e, y[e]);
+      part += (double)pairwise(t);
+    });
+    part = wave_sum(part);
+    double total = part, before = 0.0;
+    if constexpr (WAVES > 1) {
+      g.sync();
+      if (g.lane == 0) g.s.sum[g.wave] = part;
+      if (g.thread() == 0) g.s.index = -1;
+      g.sync();
+      total = 0.0;
+      for (int k = 0; k < WAVES; ++k) {
+        if (k == g.wave) before = total;
+        total += g.s.sum[k];
+      }
+    }
+    const double target = fmax(u, 0.0) * total, off = kFast ? 2.0 * bound * total : 0.0;
+    int symbol = -1;
+    float logit = 0.f;
+    bool close = false;
+    if (before <= target && target < before + part) {  // one wave
+      double run = before;
+      int last = -1;  // the wave's last entry with a weight
+      float last_logit = 0.f;
+      each([&](int j, int i, const float *y) {
+        if (symbol >= 0) return;
+        W t[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) t[e] = weight_of(j, e, y[e]);
+        const double mine = (double)pairwise(t), upto = wave_scan(mine);
+        const double chunk = lane_value(upto, kWave - 1);
+        const uint64_t pass = __ballot(run + upto > target);
+        const uint64_t some = __ballot(mine > 0.0);
+        if (some) {
+          // the first lane whose running sum passes the target, else the last with a weight;
+          // in that lane the first element that does, else its last with a weight (sums in
+          // another order can fall short of each other's borders by their rounding)
+          const int l = pass ? __builtin_ctzll(pass) : 63 - __builtin_clzll(some);
+          double c = run + (upto - mine);
+          int at = -1;
+          bool found = false, near = true;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const double next = c + (double)t[e];
+            if (!found && t[e] > (W)0) {
+              at = e;
+              found = next > target;
+              near = !(found && c < target - off && next > target + off);
+            }
+            c = next;
+          }
+          float at_logit = y[0];
+#pragma unroll
+          for (int e = 1; e < VEC; ++e) at_logit = e == at ? y[e] : at_logit;
+          last = lane_value(i + at, l);
+          last_logit = lane_value(at_logit, l);
+          if (pass) {
+            symbol = last;
+            close = lane_value(near ? 1 : 0, l) != 0;
+          }
+        }
+        run += chunk;
+      });
+      logit = last_logit;
+      if (symbol < 0) {
+        symbol = last;
+        close = true;
+      }
+      if constexpr (WAVES > 1) {
+        if (g.lane == 0) {
+          g.s.index = symbol;
+          g.s.value[0][0] = logit;
+          g.s.value[1][0] = close ? 1.f : 0.f;
+        }
+      }
+    }
+    if constexpr (WAVES > 1) {
+      g.sync();
+      symbol = g.s.index;
+      logit = g.s.value[0][0];
+      close = g.s.value[1][0] != 0.f;
+    }
+    if (symbol < 0) {  // u >= 1, or a product that rounds up to the total: the last entry with a weight
+      if (kFast) return {0, 0.f, false};
+      each([&](int j, int i, const float *y) {
+        int last = -1;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (weight_of(j, e, y[e]) > (W)0) last = i + e;
+        const uint64_t some = __ballot(last >= 0);
+        if (some) symbol = lane_value(last, 63 - __builtin_clzll(some));
+      });
+      if constexpr (WAVES > 1) {
+        g.sync();
+        if (g.lane == 0) g.s.count[g.wave] = symbol;
+        g.sync();
+        for (int k = 0; k < WAVES; ++k) symbol = max(symbol, g.s.count[k]);
+      }
+      logit = load_element<T>(row, symbol);
+    }
+    return {symbol, log_prob(logit, total), !(kFast && close)};
+  }
+
+  // (x - m) / T - log(total); the largest entry always remains, so total = 1 + the others' sum
+  __device__ __forceinline__ float log_prob(float logit, double total) const {
+    if constexpr (kFast) {
+      const float rest = (float)(total - 1.0), t = 1.0f + rest;
+      const float l = logf(t) + (rest - (t - 1.0f)) / t;
+      return (logit - m) / T_ - (rest < 1.0f ? l : logf((float)total));
+    } else {
+      return (float)(((double)logit - weight.m) / weight.T - log(total));
+    }
+  }
+};
+
+// One row: reads it, settles the rows without an answer and the greedy ones, draws from the
+// others in 32 bits and, where that is not sure, in 64.
+template <class T, int WAVES, int CHUNKS>
+__device__ __forceinline__ void sample_row(const RowGroup<WAVES> &g, const void *row, int V, double u,
+                                           float temperature, int top_k, float top_p, float min_p,
+                                           int32_t *symbol, float *log_prob) {
+  constexpr int VEC = kSampleVec<T>;
+  constexpr bool kHeld = CHUNKS > 0;
+  const int streamed = (V + WAVES * kWave * VEC - 1) / (WAVES * kWave * VEC);
+  const int chunks = kHeld ? CHUNKS : streamed;
+  float x[kHeld ? CHUNKS : 1][VEC];
+  auto first_index = [&](int j) { return ((g.wave * chunks + j) * kWave + g.lane) * VEC; };
+  float m = OT_NEG_INF, bad = 0.f;
+  auto look = [&](const float *y) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      m = fmaxf(m, y[e]);
+      if (y[e] != y[e]) bad = -1.f;
+    }
+  };
+  if constexpr (kHeld) {
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) load_logits<T>(row, first_index(j), V, x[j]);
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) look(x[j]);
+  } else {
+    for (int j = 0; j < chunks; ++j) {
+      float y[VEC];
+      load_logits<T>(row, first_index(j), V, y);
+      look(y);
+    }
+  }
+  g.extremes(m, bad);
+  Drawn d = {-1, OT_NEG_INF, true};
+  if (bad < 0.f || __builtin_isinf(m) || u != u) {
+    // no answer
+  } else if (!(temperature > 0.f)) {
+    int first = -1;
+    auto find = [&](int j, const float *y) {
+      int at = VEC;
+#pragma unroll
+      for (int e = VEC - 1; e >= 0; --e)
+        if (y[e] == m) at = e;
+      const uint64_t hit = __ballot(at < VEC);
+      if (first < 0 && hit) first = lane_value(first_index(j) + at, __builtin_ctzll(hit));
+    };
+    if constexpr (kHeld) {
+#pragma unroll
+      for (int j = 0; j < CHUNKS; ++j) find(j, x[j]);
+    } else {
+      for (int j = 0; j < chunks; ++j) {
+        float y[VEC];
+        load_logits<T>(row, first_index(j), V, y);
+        find(j, y);
+      }
+    }
+    if constexpr (WAVES > 1) {
+      g.sync();
+      if (g.lane == 0) g.s.count[g.wave] = first;
+      g.sync();
+      for (int k = WAVES - 1; k >= 0; --k)
+        if (g.s.count[k] >= 0) first = g.s.count[k];
+    }
+    d = {first, 0.f, true};
+  } else {
+    d.sure = false;
+    if (m < 1e30f && temperature >= 1e-30f && temperature <= 1e30f) {
+      const double bound = (double)((__logf((float)V) + 8.0f) * kUnit);
+      Sampler<T, WAVES, CHUNKS, FastWeight> fast(g, row, V, chunks, m, temperature, bound, x);
+      d = fast.draw(u, top_k, top_p, min_p);
+    }
+    if (!d.sure) {
+      float unused[1][VEC];
+      Sampler<T, WAVES, 0, FullWeight> full(g, row, V, streamed, m, temperature, 0.0, unused);
+      d = full.draw(u, top_k, top_p, min_p);
+    }
+  }
+  g.sync();  // the group's shared values have been read
+  if (g.thread() == 0) {
+    *symbol = d.symbol;
+    *log_prob = d.log_prob;
+  }
+}
+
+// ROWS groups of WAVES waves per workgroup, a row each
+template <class T, int WAVES, int ROWS, int CHUNKS>
+__global__ __launch_bounds__(WAVES * ROWS * kWave) void sample_kernel(
+    const void *__restrict__ logits, int64_t row_stride, int64_t rows, int V, const float *__restrict__ uniform,
+    SampleSettings set, int32_t *__restrict__ symbols, float *__restrict__ log_probs) {
+  static_assert(ROWS == 1 || WAVES == 1, "barriers are per workgroup");
+  __shared__ SampleShared<WAVES> s_row[ROWS];
+  // the wave's number in scalar registers, and with it the row and its settings
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const RowGroup<WAVES> g = {s_row[ROWS > 1 ? wave : 0], (int)(threadIdx.x % kWave), ROWS > 1 ? 0 : wave};
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + (ROWS > 1 ? wave : 0); row < rows;
+       row += (int64_t)gridDim.x * ROWS) {
+    const char *base = static_cast<const char *>(logits) + row * row_stride * (sizeof(T) == 4 ? 4 : 2);
+    sample_row<T, WAVES, CHUNKS>(g, base, V, (double)uniform[row],
+                                 set.temperature ? set.temperature[row] : set.temperature_value,
+                                 set.top_k ? set.top_k[row] : set.top_k_value,
+                                 set.top_p ? set.top_p[row] : set.top_p_value,
+                                 set.min_p ? set.min_p[row] : set.min_p_value, symbols + row, log_probs + row);
+  }
+}
+
+template <class T, int WAVES, int ROWS, int CHUNKS>
+static int launch_sample_kernel(const void *logits, int64_t row_stride, int64_t rows, int32_t V,
+                                const float *uniform, const SampleSettings &set, int32_t *symbols,
+                                float *log_probs, hipStream_t s) {
+  const int64_t groups = (rows + ROWS - 1) / ROWS;
+  const dim3 grid((unsigned)(groups < (1 << 20) ? groups : (1 << 20)));
+  hipLaunchKernelGGL((sample_kernel<T, WAVES, ROWS, CHUNKS>), grid, dim3(WAVES * ROWS * kWave), 0, s, logits,
+                     row_stride, rows, V, uniform, set, symbols, log_probs);
+  return (int)hipGetLastError();
 }
 
 template <class T>
 static int launch_sample(const void *logits, int64_t row_stride, int64_t rows, int32_t V, const float *uniform,
                          const SampleSettings &set, int32_t *symbols, float *log_probs, hipStream_t s) {
-  const dim3 grid((unsigned)(rows < (1 << 20) ? rows : (1 << 20)));
-  hipLaunchKernelGGL((sample_row_kernel<T>), grid, dim3(kBlock), 0, s, logits, row_stride, rows, V, uniform, set,
-                     symbols, log_probs);
-  return (int)hipGetLastError();
+  constexpr int VEC = kSampleVec<T>, kChunk = kWave * VEC;  // 256 or 512 elements
+#define OT_SAMPLE(WAVES_, ROWS_, CHUNKS_)                                                              \
+  return launch_sample_kernel<T, WAVES_, ROWS_, CHUNKS_>(logits, row_stride, rows, V, uniform, set, symbols, \
+                                                         log_probs, s)
+  if (V <= kChunk) OT_SAMPLE(1, 4, 1);
+  if (V <= 2 * kChunk) OT_SAMPLE(1, 4, 2);
+  if (V <= 2048) OT_SAMPLE(4, 1, 2048 / 4 / kChunk);
+  if (V <= 4096) OT_SAMPLE(4, 1, 4096 / 4 / kChunk);
+  if (V <= 6144) OT_SAMPLE(4, 1, 6144 / 4 / kChunk);
+  if (V <= 16384) OT_SAMPLE(16, 1, 16384 / 16 / kChunk);
+  if (V <= 32768) OT_SAMPLE(16, 1, 32768 / 16 / kChunk);
+  OT_SAMPLE(16, 1, 0);
+#undef OT_SAMPLE
 }
 
 }  // namespace ot
