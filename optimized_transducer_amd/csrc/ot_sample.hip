@@ -12,16 +12,11 @@
 // T = 0: the first of the largest entries, log_prob 0.  A row with no largest finite entry
 // (all -inf, a NaN, +inf) has symbol -1, log_prob -inf; so has u = NaN.
 //
-// Which index a symbol falls on, or where top_p cuts, hangs on the last bits of a sum, and the
-// answer is that of 64-bit weights and sums.  It is first looked for with 32-bit weights and a
-// bound on how far off their sums can be: only a row where a decision lies inside the bound
-// (about 4 * V * kUnit rows of one, 0.2 % at V = 500) is done again in 64 bits.
-//
-// The bound.  A 32-bit weight is off by a relative 2^-24 * |z| (the rounding of x - m, z the
-// exponent), 2^-23 (the hardware's 2^x) and 2^-24 (a last rounding); a sum of 8 adds 3 * 2^-24,
-// all longer sums are 64-bit.  Weighted with w, the |z| of a set that holds the largest entry
-// average to its entropy minus the logarithm of its total, so to ln V at most.  Any partial sum
-// is off by less than (ln V + 8) * 2^-24 of the set's total, and so is u or top_p times it.
+// Which index a symbol falls on, or where top_p cuts, hangs on the last bits of a sum: weights
+// and sums are 64-bit.  This chip's vector units do 64-bit multiply-adds at the rate of
+// (unpacked) 32-bit ones, so a weight costs 19 such instructions (a range reduction and a
+// polynomial for 2^f) where a 32-bit one through the hardware's 2^x costs 8 and the transcendental
+// unit.
 //
 // No sort: a cut is found by a histogram of the interval that still holds it, 256 bins at a
 // time, until one value is left; two levels do for rows without many equal values.
@@ -47,7 +42,6 @@ struct SampleSettings {
 };
 
 constexpr int kSampleBins = 256;
-constexpr float kUnit = 5.9604644775390625e-08f;  // 2^-24
 constexpr float kInf = __builtin_huge_valf();
 
 // ---- wave-wide helpers ----------------------------------------------------------------------
@@ -187,35 +181,29 @@ __device__ __forceinline__ void load_logits(const void *row, int i, int V, float
   }
 }
 
-// exp((x - m) / T) in 32 bits for m < 1e30 and T of [1e-30, 1e30]; c_hi + c_lo = log2(e) / T.
-// 2^(d * c) as the product's rounded part through the hardware unit and its residual to first
-// order, so that the argument's error does not grow with it.
-struct FastWeight {
-  float m, c_hi, c_lo, d_min;
-  FastWeight() = default;
-  __device__ __forceinline__ FastWeight(float m_, float T) : m(m_) {
-    constexpr float kLog2eHi = 1.44269502162933349609375f, kLog2eLo = 1.92596299112661746e-8f;
-    const float r = 1.0f / T, e = __builtin_fmaf(-T, r, 1.0f);  // 1 / T = r + r * e + ...
-    c_hi = r * kLog2eHi;
-    c_lo = __builtin_fmaf(r, kLog2eHi, -c_hi) + __builtin_fmaf(r * e, kLog2eHi, r * kLog2eLo);
-    d_min = -160.f / c_hi;  // 2^-160 is 0, and the residual of -inf would be a NaN
-  }
-  __device__ __forceinline__ float operator()(float x) const {
-    constexpr float kLn2 = 0.693147182464599609375f;
-    const float d = fmaxf(x - m, d_min);
-    const float ph = d * c_hi;
-    const float pl = __builtin_fmaf(d, c_lo, __builtin_fmaf(d, c_hi, -ph));
-    const float e = __builtin_amdgcn_exp2f(ph);
-    return __builtin_fmaf(e, pl * kLn2, e);
-  }
-};
-// the same in 64 bits, for any m and T > 0
-struct FullWeight {
-  double m, T;
-  FullWeight() = default;
-  __device__ __forceinline__ FullWeight(float m_, float T_) : m(m_), T(T_) {}
+// exp((x - m) / T) = 2^n * 2^f with n the nearest integer to (x - m) * c, c = log2(e) / T, and
+// 2^f the exponential series of f * ln 2, |f| <= 1/2, up to the 11th power (the next term is
+// below 2^-47).  Exactly 1 at x = m, exactly 0 at x = -inf.
+struct Weight {
+  double m, c;
+  __device__ __forceinline__ Weight(float m_, float T) : m(m_), c(1.4426950408889634074 / (double)T) {}
   __device__ __forceinline__ double operator()(float x) const {
-    return x == OT_NEG_INF ? 0.0 : exp(((double)x - m) / T);
+    // (T = inf and x = -inf make a NaN of the product, which fmax drops)
+    const double t = __builtin_fmax(((double)x - m) * c, -1100.0), n = __builtin_rint(t), f = t - n;
+    // ln(2)^k / k!
+    double p = 4.4455382718708115e-10;
+    p = __builtin_fma(p, f, 7.0549116208011233e-09);
+    p = __builtin_fma(p, f, 1.0178086009239699e-07);
+    p = __builtin_fma(p, f, 1.3215486790144307e-06);
+    p = __builtin_fma(p, f, 1.5252733804059841e-05);
+    p = __builtin_fma(p, f, 1.5403530393381609e-04);
+    p = __builtin_fma(p, f, 1.3333558146428443e-03);
+    p = __builtin_fma(p, f, 9.6181291076284772e-03);
+    p = __builtin_fma(p, f, 5.5504108664821580e-02);
+    p = __builtin_fma(p, f, 2.4022650695910072e-01);
+    p = __builtin_fma(p, f, 6.9314718055994531e-01);
+    p = __builtin_fma(p, f, 1.0);
+    return __builtin_ldexp(p, (int)n);
   }
 };
 
@@ -229,7 +217,6 @@ __device__ __forceinline__ unsigned order_key(float x) {
 struct Drawn {
   int symbol;
   float log_prob;
-  bool sure;
 };
 
 // Draws from a row with a finite largest entry m at a temperature above 0.  Every thread of the
@@ -237,33 +224,28 @@ struct Drawn {
 //   CHUNKS > 0: wave w holds elements [w * CHUNKS * 64 * VEC, + CHUNKS * 64 * VEC) in x, chunk by
 //     chunk, lane by lane (VEC consecutive ones each); excluded entries become -inf there
 //   CHUNKS = 0: the row is read from memory in every step; `per_wave` chunks per wave
-//   Weight: FastWeight (32 bits, with `bound` > 0) or FullWeight (64 bits)
-template <class T, int WAVES, int CHUNKS, class Weight>
+template <class T, int WAVES, int CHUNKS>
 struct Sampler {
   static constexpr int VEC = kSampleVec<T>;
   static constexpr bool kHeld = CHUNKS > 0;
-  static constexpr bool kFast = __is_same(Weight, FastWeight);
-  typedef decltype(Weight()(0.f)) W;
+  static constexpr bool kHeldWeights = kHeld && CHUNKS * VEC <= 24;  // else formed anew in each step
 
   const RowGroup<WAVES> &g;
   const void *row;
   const int V, per_wave;
   const float m, T_;
   const Weight weight;
-  const double bound;
   float (&x)[kHeld ? CHUNKS : 1][VEC];
-  bool sure = true;
-  W w[kHeld ? CHUNKS : 1][VEC];
+  double w[kHeldWeights ? CHUNKS : 1][VEC];
   // not held: entries below `floor_`, and those at it behind index `floor_last`, are excluded;
   // so are weights below least
   float floor_ = OT_NEG_INF;
   int floor_last = 0x7fffffff;
-  W least = 0;
+  double least = 0.0;
 
   __device__ __forceinline__ Sampler(const RowGroup<WAVES> &g_, const void *row_, int V_, int per_wave_, float m_,
-                                     float temperature, double bound_, float (&x_)[kHeld ? CHUNKS : 1][VEC])
-      : g(g_), row(row_), V(V_), per_wave(per_wave_), m(m_), T_(temperature), weight(m_, temperature),
-        bound(bound_), x(x_) {}
+                                     float temperature, float (&x_)[kHeld ? CHUNKS : 1][VEC])
+      : g(g_), row(row_), V(V_), per_wave(per_wave_), m(m_), T_(temperature), weight(m_, temperature), x(x_) {}
 
   __device__ __forceinline__ int chunks() const { return kHeld ? CHUNKS : per_wave; }
   __device__ __forceinline__ int first_index(int j) const {
@@ -287,13 +269,13 @@ struct Sampler {
       }
     }
   }
-  __device__ __forceinline__ W weight_of(int j, int e, float y) {
-    if constexpr (kHeld) return w[j][e];
-    const W v = weight(y);
-    return v >= least ? v : (W)0;
+  __device__ __forceinline__ double weight_of(int j, int e, float y) {
+    if constexpr (kHeldWeights) return w[j][e];
+    const double v = weight(y);
+    return v >= least ? v : 0.0;
   }
   // sum of a chunk's VEC weights, pairwise
-  __device__ __forceinline__ static W pairwise(const W v[VEC]) {
+  __device__ __forceinline__ static double pairwise(const double v[VEC]) {
     if constexpr (VEC == 4) return (v[0] + v[1]) + (v[2] + v[3]);
     else return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
   }
@@ -343,7 +325,7 @@ struct Sampler {
         for (int e = 0; e < VEC; ++e)
           if (x[j][e] < v || (x[j][e] == v && first_index(j) + e > last)) {
             x[j][e] = OT_NEG_INF;
-            w[j][e] = 0;
+            if constexpr (kHeldWeights) w[j][e] = 0.0;
           }
     } else {
       floor_last = v == floor_ ? min(last, floor_last) : last;
@@ -381,12 +363,7 @@ struct Sampler {
           if (y[e] >= lo && y[e] <= hi) {
             const int b = bin(y[e]);
             atomicAdd(&g.s.bin_count[b], 1u);
-            if (WEIGHTS) {
-              if constexpr (kFast)
-                unsafeAtomicAdd(reinterpret_cast<float *>(g.s.bin_weight) + b, (float)weight_of(j, e, y[e]));
-              else
-                unsafeAtomicAdd(&g.s.bin_weight[b], (double)weight_of(j, e, y[e]));
-            }
+            if (WEIGHTS) unsafeAtomicAdd(&g.s.bin_weight[b], weight_of(j, e, y[e]));
           }
       });
       g.sync();
@@ -398,9 +375,7 @@ struct Sampler {
       for (int q = 0; q < kPer; ++q) {
         const int b = g.lane * kPer + q;
         n[q] = g.s.bin_count[b];
-        amount[q] = !WEIGHTS ? (double)n[q]
-                    : kFast  ? (double)reinterpret_cast<const float *>(g.s.bin_weight)[b]
-                             : g.s.bin_weight[b];
+        amount[q] = WEIGHTS ? g.s.bin_weight[b] : (double)n[q];
         mine += amount[q];
       }
       double run = above + (wave_scan(mine) - mine);
@@ -479,13 +454,13 @@ struct Sampler {
     sum = 0.0;
     at_v = 0;
     each([&](int j, int, const float *y) {
-      W t[VEC];
+      double t[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        t[e] = y[e] > v ? weight_of(j, e, y[e]) : (W)0;
+        t[e] = y[e] > v ? weight_of(j, e, y[e]) : 0.0;
         at_v += y[e] == v;
       }
-      sum += (double)pairwise(t);
+      sum += pairwise(t);
     });
     g.totals(sum, at_v);
   }
@@ -499,7 +474,7 @@ struct Sampler {
     const float v = select<true>(want, smallest(), above);
     int at_v;
     sum_above(v, sum, at_v);
-    const double wv = (double)weight(v);
+    const double wv = weight(v);
     // of the entries at v, number j (from 0) remains if sum + j * wv < want
     int n = at_v;
     if (wv > 0.0) {
@@ -507,66 +482,39 @@ struct Sampler {
       n = q < 1.0 ? 0 : q < at_v ? (int)q : at_v;
     }
     if (v == m) n = max(n, 1);
-    if (kFast) {
-      const double off = 2.0 * bound * total;
-      const bool first = v == m && n == 1;  // remains whatever `want` is
-      if (!(first || (n >= 1 && sum + (n - 1) * wv < want - off)) || !(sum + n * wv >= want + off)) sure = false;
-    }
     exclude(v, n, at_v);
   }
 
   __device__ __forceinline__ void keep_min_p(float p) {
-    if constexpr (kHeld) {
-      bool near = false;
+    least = p;
+    if constexpr (kHeldWeights) {
 #pragma unroll
       for (int j = 0; j < CHUNKS; ++j)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          // a 32-bit weight is within 2^-24 * (|z| + 3) of the 64-bit one, |z| < 104 here
-          if (kFast && x[j][e] < m && __builtin_fabsf((float)w[j][e] - p) <= 128.f * kUnit * p) near = true;
-          if (!(w[j][e] >= (W)p)) w[j][e] = 0;
-        }
-      if (kFast && any(near)) sure = false;
-    } else {
-      least = (W)p;
-      if constexpr (kFast) {
-        bool near = false;
-        each([&](int, int, const float *y) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            if (y[e] < m && __builtin_fabsf((float)weight(y[e]) - p) <= 128.f * kUnit * p) near = true;
-        });
-        if (any(near)) sure = false;
-      }
+        for (int e = 0; e < VEC; ++e)
+          if (!(w[j][e] >= least)) w[j][e] = 0.0;
     }
-  }
-  __device__ __forceinline__ bool any(bool b) {
-    float hi = b ? 1.f : 0.f, lo = 0.f;
-    g.extremes(hi, lo);
-    return hi > 0.f;
   }
 
   __device__ __forceinline__ Drawn draw(double u, int top_k, float top_p, float min_p) {
     if (top_k > 0 && top_k < V) keep_top_k(top_k);
-    if constexpr (kHeld) {
+    if constexpr (kHeldWeights) {
 #pragma unroll
       for (int j = 0; j < CHUNKS; ++j)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) w[j][e] = weight(x[j][e]);
     }
     if (top_p < 1.f) keep_top_p(top_p);
-    if (kFast && !sure) return {0, 0.f, false};
     if (min_p > 0.f) keep_min_p(fminf(min_p, 1.f));
-    if (kFast && !sure) return {0, 0.f, false};
 
     // totals of the waves' parts, then the part, the chunk, the lane and the element in which
     // the running sum passes u * total
     double part = 0.0;
     each([&](int j, int, const float *y) {
-      W t[VEC];
+      double t[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) t[e] = weight_of(j, e, y[e]);
-      part += (double)pairwise(t);
+      part += pairwise(t);
     });
     part = wave_sum(part);
     double total = part, before = 0.0;
@@ -581,20 +529,19 @@ struct Sampler {
         total += g.s.sum[k];
       }
     }
-    const double target = fmax(u, 0.0) * total, off = kFast ? 2.0 * bound * total : 0.0;
+    const double target = fmax(u, 0.0) * total;
     int symbol = -1;
     float logit = 0.f;
-    bool close = false;
     if (before <= target && target < before + part) {  // one wave
       double run = before;
       int last = -1;  // the wave's last entry with a weight
       float last_logit = 0.f;
       each([&](int j, int i, const float *y) {
         if (symbol >= 0) return;
-        W t[VEC];
+        double t[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) t[e] = weight_of(j, e, y[e]);
-        const double mine = (double)pairwise(t), upto = wave_scan(mine);
+        const double mine = pairwise(t), upto = wave_scan(mine);
         const double chunk = lane_value(upto, kWave - 1);
         const uint64_t pass = __ballot(run + upto > target);
         const uint64_t some = __ballot(mine > 0.0);
@@ -605,39 +552,32 @@ struct Sampler {
           const int l = pass ? __builtin_ctzll(pass) : 63 - __builtin_clzll(some);
           double c = run + (upto - mine);
           int at = -1;
-          bool found = false, near = true;
+          bool found = false;
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            const double next = c + (double)t[e];
-            if (!found && t[e] > (W)0) {
+            const double next = c + t[e];
+            if (!found && t[e] > 0.0) {
               at = e;
               found = next > target;
-              near = !(found && c < target - off && next > target + off);
             }
             c = next;
           }
-          float at_logit = y[0];
+          // (a maximum, and not a choice between elements, which would index the registers)
+          float at_logit = OT_NEG_INF;
 #pragma unroll
-          for (int e = 1; e < VEC; ++e) at_logit = e == at ? y[e] : at_logit;
+          for (int e = 0; e < VEC; ++e) at_logit = fmaxf(at_logit, e == at ? y[e] : OT_NEG_INF);
           last = lane_value(i + at, l);
           last_logit = lane_value(at_logit, l);
-          if (pass) {
-            symbol = last;
-            close = lane_value(near ? 1 : 0, l) != 0;
-          }
+          if (pass) symbol = last;
         }
         run += chunk;
       });
       logit = last_logit;
-      if (symbol < 0) {
-        symbol = last;
-        close = true;
-      }
+      if (symbol < 0) symbol = last;
       if constexpr (WAVES > 1) {
         if (g.lane == 0) {
           g.s.index = symbol;
           g.s.value[0][0] = logit;
-          g.s.value[1][0] = close ? 1.f : 0.f;
         }
       }
     }
@@ -645,15 +585,13 @@ struct Sampler {
       g.sync();
       symbol = g.s.index;
       logit = g.s.value[0][0];
-      close = g.s.value[1][0] != 0.f;
     }
     if (symbol < 0) {  // u >= 1, or a product that rounds up to the total: the last entry with a weight
-      if (kFast) return {0, 0.f, false};
       each([&](int j, int i, const float *y) {
         int last = -1;
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
-          if (weight_of(j, e, y[e]) > (W)0) last = i + e;
+          if (weight_of(j, e, y[e]) > 0.0) last = i + e;
         const uint64_t some = __ballot(last >= 0);
         if (some) symbol = lane_value(last, 63 - __builtin_clzll(some));
       });
@@ -665,31 +603,27 @@ struct Sampler {
       }
       logit = load_element<T>(row, symbol);
     }
-    return {symbol, log_prob(logit, total), !(kFast && close)};
+    return {symbol, log_prob(logit, total)};
   }
 
   // (x - m) / T - log(total); the largest entry always remains, so total = 1 + the others' sum
   __device__ __forceinline__ float log_prob(float logit, double total) const {
-    if constexpr (kFast) {
-      const float rest = (float)(total - 1.0), t = 1.0f + rest;
-      const float l = logf(t) + (rest - (t - 1.0f)) / t;
-      return (logit - m) / T_ - (rest < 1.0f ? l : logf((float)total));
-    } else {
-      return (float)(((double)logit - weight.m) / weight.T - log(total));
-    }
+    const float rest = (float)(total - 1.0), t = 1.0f + rest;
+    const float small = logf(t) + (rest - (t - 1.0f)) / t;
+    const float z = m - logit > 3e38f || T_ < 1e-30f || T_ > 1e30f ? (float)(((double)logit - m) / T_) : (logit - m) / T_;
+    return z - (rest < 1.0f ? small : logf((float)total));
   }
 };
 
 // One row: reads it, settles the rows without an answer and the greedy ones, draws from the
-// others in 32 bits and, where that is not sure, in 64.
+// others.
 template <class T, int WAVES, int CHUNKS>
 __device__ __forceinline__ void sample_row(const RowGroup<WAVES> &g, const void *row, int V, double u,
                                            float temperature, int top_k, float top_p, float min_p,
                                            int32_t *symbol, float *log_prob) {
   constexpr int VEC = kSampleVec<T>;
   constexpr bool kHeld = CHUNKS > 0;
-  const int streamed = (V + WAVES * kWave * VEC - 1) / (WAVES * kWave * VEC);
-  const int chunks = kHeld ? CHUNKS : streamed;
+  const int chunks = kHeld ? CHUNKS : (V + WAVES * kWave * VEC - 1) / (WAVES * kWave * VEC);
   float x[kHeld ? CHUNKS : 1][VEC];
   auto first_index = [&](int j) { return ((g.wave * chunks + j) * kWave + g.lane) * VEC; };
   float m = OT_NEG_INF, bad = 0.f;
@@ -713,7 +647,7 @@ __device__ __forceinline__ void sample_row(const RowGroup<WAVES> &g, const void 
     }
   }
   g.extremes(m, bad);
-  Drawn d = {-1, OT_NEG_INF, true};
+  Drawn d = {-1, OT_NEG_INF};
   if (bad < 0.f || __builtin_isinf(m) || u != u) {
     // no answer
   } else if (!(temperature > 0.f)) {
@@ -743,19 +677,10 @@ __device__ __forceinline__ void sample_row(const RowGroup<WAVES> &g, const void 
       for (int k = WAVES - 1; k >= 0; --k)
         if (g.s.count[k] >= 0) first = g.s.count[k];
     }
-    d = {first, 0.f, true};
+    d = {first, 0.f};
   } else {
-    d.sure = false;
-    if (m < 1e30f && temperature >= 1e-30f && temperature <= 1e30f) {
-      const double bound = (double)((__logf((float)V) + 8.0f) * kUnit);
-      Sampler<T, WAVES, CHUNKS, FastWeight> fast(g, row, V, chunks, m, temperature, bound, x);
-      d = fast.draw(u, top_k, top_p, min_p);
-    }
-    if (!d.sure) {
-      float unused[1][VEC];
-      Sampler<T, WAVES, 0, FullWeight> full(g, row, V, streamed, m, temperature, 0.0, unused);
-      d = full.draw(u, top_k, top_p, min_p);
-    }
+    Sampler<T, WAVES, CHUNKS> sampler(g, row, V, chunks, m, temperature, x);
+    d = sampler.draw(u, top_k, top_p, min_p);
   }
   g.sync();  // the group's shared values have been read
   if (g.thread() == 0) {
@@ -766,7 +691,7 @@ __device__ __forceinline__ void sample_row(const RowGroup<WAVES> &g, const void 
 
 // ROWS groups of WAVES waves per workgroup, a row each
 template <class T, int WAVES, int ROWS, int CHUNKS>
-__global__ __launch_bounds__(WAVES * ROWS * kWave) void sample_kernel(
+__global__ __launch_bounds__(WAVES * ROWS * kWave, 4) void sample_kernel(
     const void *__restrict__ logits, int64_t row_stride, int64_t rows, int V, const float *__restrict__ uniform,
     SampleSettings set, int32_t *__restrict__ symbols, float *__restrict__ log_probs) {
   static_assert(ROWS == 1 || WAVES == 1, "barriers are per workgroup");
