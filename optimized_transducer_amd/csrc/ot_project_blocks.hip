@@ -30,7 +30,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kBlocksK = 128;      // elements per scale
 constexpr int kBlocksUnit = 16;    // D is a multiple of this: one 16-byte load
-constexpr int kPartCols = 64;      // vocabulary entries behind one partial log-sum-exp
+constexpr int kSmallCols = 64;     // vocabulary entries of a workgroup of the small kernel
+constexpr int kPartCols = 16;      // least vocabulary entries behind one partial log-sum-exp
 
 // a running log-sum-exp as (largest value, sum of exp(value - largest))
 struct LogSum {
@@ -97,7 +98,7 @@ __global__ __launch_bounds__(kBlock) void project_blocks_small_kernel(
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int64_t row0 = tile / col_tiles * 16;
     const int part = (int)(tile % col_tiles);
-    const int v0 = part * kPartCols + wave * 16;
+    const int v0 = part * kSmallCols + wave * 16;
     const int64_t row = row0 + r;
     const bool row_in = row < rows;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -144,6 +145,199 @@ __global__ __launch_bounds__(kBlock) void project_blocks_small_kernel(
   }
 }
 
+// 4 consecutive logits of a row; the row may start anywhere its type can
+template <class T>
+__device__ __forceinline__ void store_logits4(void *logits, int64_t i, const float y[4]) {
+  if constexpr (sizeof(T) == 4) {
+    typedef f32x4 unaligned __attribute__((aligned(4)));
+    const f32x4 t = {y[0], y[1], y[2], y[3]};
+    *reinterpret_cast<unaligned *>(static_cast<float *>(logits) + i) = t;
+  } else {
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    typedef u32x2 unaligned __attribute__((aligned(2)));
+    const u32x2 t = {(unsigned)from_float<T>(y[0]) | ((unsigned)from_float<T>(y[1]) << 16),
+                     (unsigned)from_float<T>(y[2]) | ((unsigned)from_float<T>(y[3]) << 16)};
+    *reinterpret_cast<unaligned *>(static_cast<unsigned short *>(logits) + i) = t;
+  }
+}
+
+// Many rows.  A workgroup of 4 waves owns 64 * TILES packed rows; a wave holds its 16 * TILES
+// rows of x, widened, in registers for the whole walk over the vocabulary, so x is read and
+// widened once.  The weight goes by in stages of COLS vocabulary entries (8-bit, all of D)
+// through two LDS buffers: the next stage's global loads are in flight while a stage is
+// multiplied, and are written to the other buffer behind it.  16-byte slots of LDS are
+// XOR-swizzled by their row against bank conflicts.
+//   KB: blocks of 128 in D that registers are laid out for (D may have fewer)
+// Lane l holds bytes [64 q + 16 (l / 16), + 16) of a block of row l % 16 (q = 0, 1); the first 8
+// feed matrix instruction 2 q and the others 2 q + 1, in both operands alike.
+template <class T, int KB, int TILES, int COLS, int WAVES_PER_SIMD>
+__global__ __launch_bounds__(kBlock, WAVES_PER_SIMD) void project_blocks_kernel(
+    const unsigned char *__restrict__ x, const float *__restrict__ xs, const unsigned char *__restrict__ w,
+    const float *__restrict__ ws, const float *__restrict__ bias, int64_t rows, int D, int V,
+    int stages_per_part, void *__restrict__ logits, float *__restrict__ den, LogSum *__restrict__ parts) {
+  constexpr int kRowBytes = KB * kBlocksK, kSlots = kRowBytes / 16;
+  constexpr int kPieces = COLS * kSlots / kBlock;  // 16-byte pieces of a stage per thread
+  static_assert(kPieces * kBlock == COLS * kSlots && COLS % 16 == 0 && kBlocksK % COLS == 0, "");
+  __shared__ __attribute__((aligned(16))) unsigned char s_w[2][COLS * kRowBytes];
+  __shared__ __attribute__((aligned(16))) float s_bias[2][COLS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int r = lane & 15, h = lane >> 4;
+  const int nblocks = (D + kBlocksK - 1) / kBlocksK;
+  const int stages = (V + COLS - 1) / COLS;
+  const int part = blockIdx.y;
+  const int stage0 = part * stages_per_part, stage1 = min(stages, stage0 + stages_per_part);
+
+  // this thread's pieces of a stage: row, slot and place in LDS
+  i32x4 piece[kPieces];
+  float piece_bias;
+  auto load_stage = [&](int stage) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int p = tid + i * kBlock, row = p / kSlots, slot = p % kSlots;
+      const int v = min(stage * COLS + row, V - 1);  // entries past the end are masked later
+      piece[i] = i32x4{0, 0, 0, 0};
+      if (slot * 16 < D) piece[i] = *reinterpret_cast<const i32x4 *>(w + (int64_t)v * D + slot * 16);
+    }
+    if (tid < COLS) {
+      const int v = stage * COLS + tid;
+      piece_bias = v < V ? (bias ? bias[v] : 0.f) : OT_NEG_INF;
+    }
+  };
+  auto store_stage = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int p = tid + i * kBlock, row = p / kSlots, slot = p % kSlots;
+      *reinterpret_cast<i32x4 *>(&s_w[buf][row * kRowBytes + ((slot ^ (row & 7)) * 16)]) = piece[i];
+    }
+    if (tid < COLS) s_bias[buf][tid] = piece_bias;
+  };
+
+  load_stage(stage0);
+  // x: 16 * TILES rows per wave
+  const int64_t row0 = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * (64 * TILES) + wave * (16 * TILES);
+  bf16x8 xf[TILES][KB][4];
+  float xscale[TILES][KB];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    const int64_t row = min(row0 + 16 * t + r, rows - 1);
+    const unsigned char *xr = x + row * D;
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      xscale[t][b] = b < nblocks ? xs[row * nblocks + b] : 0.f;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int k = b * kBlocksK + 64 * q + 16 * h;
+        i32x4 c = {0, 0, 0, 0};
+        if (k < D) c = *reinterpret_cast<const i32x4 *>(xr + k);
+        xf[t][b][2 * q] = widen(c[0], c[1]);
+        xf[t][b][2 * q + 1] = widen(c[2], c[3]);
+      }
+    }
+  }
+  store_stage(0);
+
+  // running log-sum-exp of this lane's share of its rows, relative to ref: ref follows the
+  // largest value so far at a distance of at most 20, so that few values make it move
+  float ref[TILES], sum[TILES];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    ref[t] = OT_NEG_INF;
+    sum[t] = 0.f;
+  }
+  const bool want_den = den || parts;
+
+  for (int stage = stage0; stage < stage1; ++stage) {
+    const int buf = (stage - stage0) & 1;
+    lds_barrier();  // LDS only: the logits' stores stay in flight
+    if (stage + 1 < stage1) load_stage(stage + 1);
+    // the stage lies in one block of 128 vocabulary entries
+    const float *wsr = ws + (int64_t)(stage * COLS / kBlocksK) * nblocks;
+    float scale[TILES][KB];
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      const float sw = b < nblocks ? wsr[b] : 0.f;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) scale[t][b] = xscale[t][b] * sw;
+    }
+#pragma unroll 1
+    for (int c = 0; c < COLS / 16; ++c) {
+      const int v0 = stage * COLS + 16 * c;
+      if (v0 >= V) break;
+      const f32x4 b4 = *reinterpret_cast<const f32x4 *>(&s_bias[buf][16 * c + 4 * h]);
+      f32x4 acc[TILES];
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) acc[t] = b4;
+      const unsigned char *wr = &s_w[buf][(16 * c + r) * kRowBytes];
+#pragma unroll
+      for (int b = 0; b < KB; ++b) {
+        if (KB > 4 && b >= nblocks) continue;
+        f32x4 p[TILES];
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const i32x4 d = *reinterpret_cast<const i32x4 *>(wr + (((b * 8 + 4 * q + h) ^ (r & 7)) * 16));
+          const bf16x8 w0 = widen(d[0], d[1]), w1 = widen(d[2], d[3]);
+#pragma unroll
+          for (int t = 0; t < TILES; ++t)
+            p[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w0, xf[t][b][2 * q], p[t], 0, 0, 0);
+#pragma unroll
+          for (int t = 0; t < TILES; ++t)
+            p[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w1, xf[t][b][2 * q + 1], p[t], 0, 0, 0);
+        }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(p[t][i], scale[t][b], acc[t][i]);
+      }
+      // register i: vocabulary entry v0 + 4 h + i of row 16 t + r
+      const int v = v0 + 4 * h;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = v0 + 16 <= V || v + i < V ? acc[t][i] : OT_NEG_INF;
+        const int64_t row = row0 + 16 * t + r;
+        if (row < rows) {
+          if (v + 4 <= V) {
+            store_logits4<T>(logits, row * V + v, y);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (v + i < V) store_logit<T>(logits, row * V + v + i, y[i]);
+          }
+        }
+        if (want_den) {
+          constexpr float kLog2e = 1.44269502162933349609375f;
+          const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+          if (top > ref[t] + 20.f) {
+            if (sum[t] != 0.f) sum[t] *= expf(ref[t] - top);
+            ref[t] = top;
+          }
+          const float shift = __builtin_isinf(ref[t]) ? 0.f : -ref[t];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[t] += __builtin_amdgcn_exp2f((y[i] + shift) * kLog2e);
+        }
+      }
+    }
+    if (stage + 1 < stage1) store_stage(buf ^ 1);
+  }
+  if (!want_den) return;
+  // the four lanes of a row meet
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    LogSum run = {ref[t], sum[t]};
+#pragma unroll
+    for (int d = 16; d < 64; d *= 2)
+      run = merge(run, {__shfl_xor(run.m, d, kWave), __shfl_xor(run.s, d, kWave)});
+    const int64_t row = row0 + 16 * t + r;
+    if (h == 0 && row < rows) {
+      if (parts) parts[(int64_t)part * rows + row] = run;
+      else den[row] = logf(run.s) + (__builtin_isinf(run.m) ? 0.f : run.m);
+    }
+  }
+}
+
 // den[r] = log-sum-exp of a row's parts, merged in order
 __global__ __launch_bounds__(kBlock) void project_blocks_den_kernel(const LogSum *__restrict__ parts,
                                                                    int nparts, int64_t rows,
@@ -155,11 +349,54 @@ __global__ __launch_bounds__(kBlock) void project_blocks_den_kernel(const LogSum
   den[r] = logf(t.s) + (__builtin_isinf(t.m) ? 0.f : t.m);
 }
 
+template <class T, int KB, int TILES, int COLS, int WAVES_PER_SIMD>
+static int launch_project_blocks_kernel(const unsigned char *x, const float *xs, const unsigned char *w,
+                                        const float *ws, const float *bias, int64_t rows, int32_t D, int32_t V,
+                                        void *logits, float *den, LogSum *parts, int cus, hipStream_t s) {
+  const int64_t row_groups = (rows + 64 * TILES - 1) / (64 * TILES);
+  // the vocabulary is dealt out to several workgroups where the rows alone do not fill the chip
+  const int stages = (V + COLS - 1) / COLS;
+  const int64_t wanted = (int64_t)cus * WAVES_PER_SIMD;
+  int64_t split = row_groups >= wanted ? 1 : (wanted + row_groups - 1) / row_groups;
+  if (split > stages) split = stages;
+  const int stages_per_part = (int)((stages + split - 1) / split);
+  const int nparts = (stages + stages_per_part - 1) / stages_per_part;
+  const bool merged = den && nparts > 1;
+  // (a launch holds 2^32 threads at most in each direction)
+  constexpr int64_t kMostX = 1 << 20;
+  const dim3 grid((unsigned)(row_groups < kMostX ? row_groups : kMostX), (unsigned)nparts,
+                  (unsigned)((row_groups + kMostX - 1) / kMostX));
+  hipLaunchKernelGGL((project_blocks_kernel<T, KB, TILES, COLS, WAVES_PER_SIMD>),
+                     grid, dim3(kBlock), 0, s, x, xs, w, ws, bias, rows, D, V, stages_per_part, logits,
+                     merged ? nullptr : den, merged ? parts : nullptr);
+  if (merged)
+    hipLaunchKernelGGL(project_blocks_den_kernel, dim3((unsigned)((rows + kBlock - 1) / kBlock)), dim3(kBlock),
+                       0, s, parts, nparts, rows, den);
+  return (int)hipGetLastError();
+}
+
 template <class T>
 static int launch_project_blocks(const unsigned char *x, const float *xs, const unsigned char *w,
                                  const float *ws, const float *bias, int64_t rows, int32_t D, int32_t V,
                                  void *logits, float *den, LogSum *parts, hipStream_t s) {
-  const int col_tiles = (V + kPartCols - 1) / kPartCols;
+  int device = 0, cus = 0;
+  if (hipGetDevice(&device) != hipSuccess ||
+      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || cus <= 0)
+    return OT_E_BAD_ARG;
+  const int nblocks = (D + kBlocksK - 1) / kBlocksK;
+  if (rows > 64 && nblocks <= 16) {
+#define OT_PROJECT(KB_, TILES_, COLS_, WAVES_)                                                              \
+  return launch_project_blocks_kernel<T, KB_, TILES_, COLS_, WAVES_>(x, xs, w, ws, bias, rows, D, V, logits, \
+                                                                     den, parts, cus, s)
+    if (nblocks == 1) OT_PROJECT(1, 2, 64, 2);
+    if (nblocks == 2) OT_PROJECT(2, 2, 64, 2);
+    if (nblocks == 3) OT_PROJECT(3, 2, 32, 2);
+    if (nblocks == 4) OT_PROJECT(4, 2, 32, 2);
+    if (nblocks <= 8) OT_PROJECT(8, 2, 32, 1);
+    OT_PROJECT(16, 1, 16, 1);
+#undef OT_PROJECT
+  }
+  const int col_tiles = (V + kSmallCols - 1) / kSmallCols;
   const int64_t tiles = (rows + 15) / 16 * col_tiles;
   const dim3 grid((unsigned)(tiles < (1 << 22) ? tiles : (1 << 22)));
   hipLaunchKernelGGL((project_blocks_small_kernel<T>), grid, dim3(kBlock), 0, s, x, xs, w, ws, bias, rows, D,
