@@ -24,6 +24,7 @@ namespace ot {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -31,6 +32,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 constexpr int kBlocksK = 128;      // elements per scale
 constexpr int kBlocksUnit = 16;    // D is a multiple of this: one 16-byte load
 constexpr int kSmallCols = 64;     // vocabulary entries of a workgroup of the small kernel
+constexpr int kWideCols = 32;      // vocabulary entries of a stage of the wide kernel
 constexpr int kPartCols = 16;      // least vocabulary entries behind one partial log-sum-exp
 
 // a running log-sum-exp as (largest value, sum of exp(value - largest))
@@ -153,7 +155,6 @@ __device__ __forceinline__ void store_logits4(void *logits, int64_t i, const flo
     const f32x4 t = {y[0], y[1], y[2], y[3]};
     *reinterpret_cast<unaligned *>(static_cast<float *>(logits) + i) = t;
   } else {
-    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
     typedef u32x2 unaligned __attribute__((aligned(2)));
     const u32x2 t = {(unsigned)from_float<T>(y[0]) | ((unsigned)from_float<T>(y[1]) << 16),
                      (unsigned)from_float<T>(y[2]) | ((unsigned)from_float<T>(y[3]) << 16)};
@@ -338,6 +339,261 @@ __global__ __launch_bounds__(kBlock, WAVES_PER_SIMD) void project_blocks_kernel(
   }
 }
 
+// Many rows of up to KB blocks.  A workgroup of 4 waves owns 64 * TILES packed rows; a wave holds
+// its 16 * TILES rows of x, widened, in registers for the whole walk over the vocabulary, so x is
+// read and widened once.  The weight goes by in stages of 32 vocabulary entries (all of D, 8-bit)
+// through two LDS buffers: the next stage's global loads are issued at the start of a stage and
+// written in its last part, with one barrier per stage.  16-byte slots of LDS are XOR-swizzled by
+// their row against bank conflicts.
+//
+// The walk advances in steps of 16 vocabulary entries x one block (4 * TILES matrix instructions);
+// the LDS read of a step's weight is issued one step ahead.  Nothing in a step branches: rows past
+// the end are dropped by the bounds of the store's buffer view, entries past the end have weight 0
+// and a starting value of -inf.
+//
+// Which entry of the vocabulary a row of the accumulator tile stands for is free: it is chosen so
+// that a lane ends up with 16 bytes of consecutive logits and four lanes with 64, from one group of
+// 16 entries for 4-byte logits and from two for 2-byte ones.
+//   ALIGNED: 4 logits start at a multiple of 4 bytes (else 2-byte logits are stored one by one)
+// Lane l holds bytes [64 q + 16 (l / 16), + 16) of a block of row l % 16 (q = 0, 1); the first 8
+// feed matrix instruction 2 q and the others 2 q + 1, in both operands alike.
+template <class T, int KB, int TILES, int WAVES_PER_SIMD, bool ALIGNED, bool DEN>
+__global__ __launch_bounds__(kBlock, WAVES_PER_SIMD) void project_blocks_wide_kernel(
+    const unsigned char *__restrict__ x, const float *__restrict__ xs, const unsigned char *__restrict__ w,
+    const float *__restrict__ ws, const float *__restrict__ bias, int64_t rows, int D, int V,
+    int stages_per_part, void *__restrict__ logits, float *__restrict__ den, LogSum *__restrict__ parts) {
+  constexpr int kCols = kWideCols;
+  constexpr int kSlots = KB * 8;                    // 16-byte slots of a row
+  constexpr int kPieces = kCols * kSlots / kBlock;  // of a stage per thread
+  constexpr int kLdsSlots = kCols * kSlots + 8 * (kCols / 8);  // of a stage, padded (see place())
+  constexpr unsigned kOut = sizeof(T) == 4 ? 4u : 2u;
+  constexpr int kGroup = 16 / (int)kOut;            // consecutive entries of a lane
+  constexpr int kSubs = kGroup / 4;                 // groups of 16 entries behind them
+  constexpr unsigned kNowhere = 0xffffffe0u;        // an offset that a store drops
+  static_assert(kPieces * kBlock == kCols * kSlots, "");
+  __shared__ __attribute__((aligned(16))) i32x4 s_w[2][kLdsSlots];
+  __shared__ __attribute__((aligned(16))) float s_bias[2][kCols];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int r = lane & 15, h = lane >> 4;
+  const int nblocks = (D + kBlocksK - 1) / kBlocksK;
+  const int stages = (V + kCols - 1) / kCols;
+  const int part = blockIdx.y;
+  const int stage0 = part * stages_per_part, stage1 = min(stages, stage0 + stages_per_part);
+
+  // Place of a 16-byte slot of a stage's row in LDS.  A 16-byte read is served 16 lanes at a time:
+  // lanes 0-7 and 24-31 of a half-wave, or 8-23, that is r < 8 of one h and r >= 8 of the other.
+  // Three bits of the row that lane r reads (r & 7) spread 8 lanes over 128 bytes; the other 8 are
+  // half of the 256 bytes that the banks hold away, by a pad of 128 bytes every 8 rows of r.
+  auto place = [&](int row, int slot) -> int {
+    const int lane8 = kSubs == 1 ? row & 7 : (row & 3) | ((row >> 1) & 4);
+    const int half = kSubs == 1 ? row >> 3 : row >> 4;
+    return row * kSlots + (KB % 2 == 0 ? 8 * half : 0) + (slot ^ lane8);
+  };
+  i32x4 piece[kPieces];
+  float piece_bias = 0.f;
+  auto load_stage = [&](int stage) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int p = tid + i * kBlock, row = p / kSlots, slot = p % kSlots;
+      const int v = stage * kCols + row;
+      piece[i] = i32x4{0, 0, 0, 0};
+      if (slot * 16 < D && v < V) piece[i] = *reinterpret_cast<const i32x4 *>(w + (int64_t)v * D + slot * 16);
+    }
+    if (tid < kCols) {
+      const int v = stage * kCols + tid;
+      piece_bias = v < V ? (bias ? bias[v] : 0.f) : OT_NEG_INF;
+    }
+  };
+  auto store_stage = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int p = tid + i * kBlock, row = p / kSlots, slot = p % kSlots;
+      s_w[buf][place(row, slot)] = piece[i];
+    }
+    if (tid < kCols) s_bias[buf][tid] = piece_bias;
+  };
+
+  load_stage(stage0);
+  const int64_t group0 = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * (64 * TILES);
+  if (group0 >= rows) return;
+  const int64_t row0 = group0 + wave * (16 * TILES);
+  bf16x8 xf[TILES][KB][4];
+  float xscale[TILES][KB];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    const int64_t row = min(row0 + 16 * t + r, rows - 1);
+    const unsigned char *xr = x + row * D;
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      xscale[t][b] = b < nblocks ? xs[row * nblocks + b] : 0.f;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int k = b * kBlocksK + 64 * q + 16 * h;
+        i32x4 c = {0, 0, 0, 0};
+        if (k < D) c = *reinterpret_cast<const i32x4 *>(xr + k);
+        xf[t][b][2 * q] = widen(c[0], c[1]);
+        xf[t][b][2 * q + 1] = widen(c[2], c[3]);
+      }
+    }
+  }
+  store_stage(0);
+  lds_barrier();
+
+  // this workgroup's logits; a lane's byte offset of row t at its first entry of a stage
+  const __amdgpu_buffer_rsrc_t out =
+      make_buffer(static_cast<char *>(logits) + group0 * V * kOut,
+                  (unsigned)min((int64_t)(64 * TILES), rows - group0) * (unsigned)V * kOut);
+  const unsigned out_row = ((unsigned)(wave * (16 * TILES) + r) * (unsigned)V + (unsigned)(kGroup * h)) * kOut;
+  const unsigned out_tile = 16u * (unsigned)V * kOut;
+
+  // running log-sum-exp of this lane's share of its rows, relative to ref, which follows the
+  // largest value so far at a distance of at most 20
+  constexpr float kLog2e = 1.44269502162933349609375f;
+  float ref[TILES], sum[TILES];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    ref[t] = -1e30f;
+    sum[t] = 0.f;
+  }
+
+  // Row m = 4 h + i of the tile of group `sub` stands for entry kGroup * h + 4 * sub + i of the
+  // 16 * kSubs entries.  As an operand row it is lane r = m.
+  const int entry0 = kGroup * (r >> 2) + (r & 3);
+  // slot 4 q + h of a block, swizzled by the entry's row in LDS: its low three bits
+  auto weight_at = [&](int sub, int q) -> const i32x4 * {
+    return &s_w[0][place(entry0 + 4 * sub, 4 * q + h)];
+  };
+  const i32x4 *read_at[kSubs][2];
+#pragma unroll
+  for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) read_at[sub][q] = weight_at(sub, q);
+  // step (group of 16 entries `g` of the stage, block b) of buffer buf
+  auto read_weight = [&](int buf, int g, int b, i32x4 (&f)[2]) {
+    const int at = buf * kLdsSlots + (kSubs == 1 && g == 1 ? place(16, 0) : 0) + 8 * b;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) f[q] = read_at[g % kSubs][q][at];
+  };
+
+  i32x4 raw[2][2];  // weight of a step and of the next one
+  read_weight(0, 0, 0, raw[0]);
+  float scale[TILES][KB];
+  for (int stage = stage0; stage < stage1; ++stage) {
+    const int buf = (stage - stage0) & 1;
+    const bool more = stage + 1 < stage1;
+    if (more) load_stage(stage + 1);
+    {  // the stage lies in one block of 128 vocabulary entries
+      const float *wsr = ws + (int64_t)(stage * kCols / kBlocksK) * nblocks;
+#pragma unroll
+      for (int c = 0; c < KB; ++c) {
+        const float sw = c < nblocks ? wsr[c] : 0.f;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) scale[t][c] = xscale[t][c] * sw;
+      }
+    }
+#pragma unroll
+    for (int set = 0; set < kCols / (16 * kSubs); ++set) {
+      f32x4 acc[kSubs][TILES];
+#pragma unroll
+      for (int sub = 0; sub < kSubs; ++sub) {
+        const int g = set * kSubs + sub;
+        if (g == kCols / 16 - 1 && more) store_stage(buf ^ 1);
+        const f32x4 start =
+            *reinterpret_cast<const f32x4 *>(&s_bias[buf][16 * kSubs * set + kGroup * h + 4 * sub]);
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          const int cur = (g * KB + b) & 1;  // (a stage has an even number of steps)
+          // the next step's weight; behind the last step of a stage lies the barrier
+          if (b + 1 < KB) read_weight(buf, g, b + 1, raw[cur ^ 1]);
+          else if (g + 1 < kCols / 16) read_weight(buf, g + 1, 0, raw[cur ^ 1]);
+          else {
+            lds_barrier();
+            read_weight(buf ^ 1, 0, 0, raw[cur ^ 1]);
+          }
+          f32x4 p[TILES];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const i32x4 d = raw[cur][i / 2];
+            const bf16x8 wf = i & 1 ? widen(d[2], d[3]) : widen(d[0], d[1]);
+            const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+              p[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xf[t][b][i], i == 0 ? zero : p[t], 0, 0, 0);
+          }
+#pragma unroll
+          for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              acc[sub][t][i] = __builtin_fmaf(p[t][i], scale[t][b], b == 0 ? start[i] : acc[sub][t][i]);
+        }
+      }
+      // rounding, store, log-sum-exp
+      const int v0 = stage * kCols + 16 * kSubs * set;  // this lane: entries v0 + kGroup * h, + kGroup
+      const int v = v0 + kGroup * h;
+      const unsigned at = v + kGroup <= V ? out_row + (unsigned)v0 * kOut : kNowhere;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        const unsigned to = at == kNowhere ? kNowhere : at + t * out_tile;
+        if constexpr (kOut == 4) {
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[0][t]), out, to, 0, 0);
+        } else {
+          unsigned short e[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) e[i] = from_float<T>(acc[i / 4][t][i % 4]);
+          if constexpr (ALIGNED) {
+            u32x4 four;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) four[i] = (unsigned)e[2 * i] | ((unsigned)e[2 * i + 1] << 16);
+            __builtin_amdgcn_raw_buffer_store_b128(four, out, to, 0, 0);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) __builtin_amdgcn_raw_buffer_store_b16(e[i], out, to + 2 * i, 0, 0);
+          }
+        }
+      }
+      if (v0 + 16 * kSubs > V && v < V && v + kGroup > V) {  // the lane whose entries V cuts
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+          const int64_t row = row0 + 16 * t + r;
+#pragma unroll
+          for (int i = 0; i < kGroup - 1; ++i)
+            if (v + i < V && row < rows) store_logit<T>(logits, row * V + v + i, acc[i / 4][t][i % 4]);
+        }
+      }
+      if constexpr (DEN) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+          float top = acc[0][t][0];
+#pragma unroll
+          for (int i = 1; i < kGroup; ++i) top = fmaxf(top, acc[i / 4][t][i % 4]);
+          const float to = top > ref[t] + 20.f ? fminf(top, 3e38f) : ref[t];
+          float s = sum[t] * __builtin_amdgcn_exp2f((ref[t] - to) * kLog2e);
+          // (a difference first: in powers of 2 the rounding of a large `to` would be an exponent)
+#pragma unroll
+          for (int i = 0; i < kGroup; ++i) s += __builtin_amdgcn_exp2f((acc[i / 4][t][i % 4] - to) * kLog2e);
+          sum[t] = s;
+          ref[t] = to;
+        }
+      }
+    }
+  }
+  if constexpr (DEN) {
+    // the four lanes of a row meet
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      LogSum run = {ref[t], sum[t]};
+#pragma unroll
+      for (int d = 16; d < 64; d *= 2)
+        run = merge(run, {__shfl_xor(run.m, d, kWave), __shfl_xor(run.s, d, kWave)});
+      const int64_t row = row0 + 16 * t + r;
+      if (h == 0 && row < rows) {
+        if (parts) parts[(int64_t)part * rows + row] = run;
+        else den[row] = logf(run.s) + (__builtin_isinf(run.m) ? 0.f : run.m);
+      }
+    }
+  }
+}
+
 // den[r] = log-sum-exp of a row's parts, merged in order
 __global__ __launch_bounds__(kBlock) void project_blocks_den_kernel(const LogSum *__restrict__ parts,
                                                                    int nparts, int64_t rows,
@@ -349,29 +605,60 @@ __global__ __launch_bounds__(kBlock) void project_blocks_den_kernel(const LogSum
   den[r] = logf(t.s) + (__builtin_isinf(t.m) ? 0.f : t.m);
 }
 
+// Workgroups of a launch: a part of the vocabulary for each where the rows alone do not fill the
+// chip, with the denominators merged from the parts.
+struct ProjectGrid {
+  dim3 grid;
+  int stages_per_part, nparts;
+  ProjectGrid(int64_t row_groups, int64_t stages, int64_t wanted) {
+    int64_t split = row_groups >= wanted ? 1 : (wanted + row_groups - 1) / row_groups;
+    if (split > stages) split = stages;
+    stages_per_part = (int)((stages + split - 1) / split);
+    nparts = (int)((stages + stages_per_part - 1) / stages_per_part);
+    // (a launch holds 2^32 threads at most in each direction)
+    constexpr int64_t kMostX = 1 << 20;
+    grid = dim3((unsigned)(row_groups < kMostX ? row_groups : kMostX), (unsigned)nparts,
+                (unsigned)((row_groups + kMostX - 1) / kMostX));
+  }
+};
+
 template <class T, int KB, int TILES, int COLS, int WAVES_PER_SIMD>
 static int launch_project_blocks_kernel(const unsigned char *x, const float *xs, const unsigned char *w,
                                         const float *ws, const float *bias, int64_t rows, int32_t D, int32_t V,
                                         void *logits, float *den, LogSum *parts, int cus, hipStream_t s) {
-  const int64_t row_groups = (rows + 64 * TILES - 1) / (64 * TILES);
-  // the vocabulary is dealt out to several workgroups where the rows alone do not fill the chip
-  const int stages = (V + COLS - 1) / COLS;
-  const int64_t wanted = (int64_t)cus * WAVES_PER_SIMD;
-  int64_t split = row_groups >= wanted ? 1 : (wanted + row_groups - 1) / row_groups;
-  if (split > stages) split = stages;
-  const int stages_per_part = (int)((stages + split - 1) / split);
-  const int nparts = (stages + stages_per_part - 1) / stages_per_part;
-  const bool merged = den && nparts > 1;
-  // (a launch holds 2^32 threads at most in each direction)
-  constexpr int64_t kMostX = 1 << 20;
-  const dim3 grid((unsigned)(row_groups < kMostX ? row_groups : kMostX), (unsigned)nparts,
-                  (unsigned)((row_groups + kMostX - 1) / kMostX));
+  const ProjectGrid g((rows + 64 * TILES - 1) / (64 * TILES), (V + COLS - 1) / COLS, (int64_t)cus * WAVES_PER_SIMD);
+  const bool merged = den && g.nparts > 1;
   hipLaunchKernelGGL((project_blocks_kernel<T, KB, TILES, COLS, WAVES_PER_SIMD>),
-                     grid, dim3(kBlock), 0, s, x, xs, w, ws, bias, rows, D, V, stages_per_part, logits,
+                     g.grid, dim3(kBlock), 0, s, x, xs, w, ws, bias, rows, D, V, g.stages_per_part, logits,
                      merged ? nullptr : den, merged ? parts : nullptr);
   if (merged)
     hipLaunchKernelGGL(project_blocks_den_kernel, dim3((unsigned)((rows + kBlock - 1) / kBlock)), dim3(kBlock),
-                       0, s, parts, nparts, rows, den);
+                       0, s, parts, g.nparts, rows, den);
+  return (int)hipGetLastError();
+}
+
+template <class T, int KB, int TILES, int WAVES_PER_SIMD>
+static int launch_project_blocks_wide(const unsigned char *x, const float *xs, const unsigned char *w,
+                                      const float *ws, const float *bias, int64_t rows, int32_t D, int32_t V,
+                                      void *logits, float *den, LogSum *parts, int cus, hipStream_t s) {
+  const ProjectGrid g((rows + 64 * TILES - 1) / (64 * TILES), (V + kWideCols - 1) / kWideCols,
+                      (int64_t)cus * WAVES_PER_SIMD);
+  const bool merged = den && g.nparts > 1;
+#define OT_WIDE(ALIGNED_, DEN_)                                                                             \
+  hipLaunchKernelGGL((project_blocks_wide_kernel<T, KB, TILES, WAVES_PER_SIMD, ALIGNED_, DEN_>), g.grid, dim3(kBlock), 0, s, \
+                     x, xs, w, ws, bias, rows, D, V, g.stages_per_part, logits, merged ? nullptr : den,      \
+                     merged ? parts : nullptr)
+  if (sizeof(T) == 4 || (V % 2 == 0 && (reinterpret_cast<uintptr_t>(logits) & 3) == 0)) {
+    if (den) OT_WIDE(true, true);
+    else OT_WIDE(true, false);
+  } else if constexpr (sizeof(T) != 4) {
+    if (den) OT_WIDE(false, true);
+    else OT_WIDE(false, false);
+  }
+#undef OT_WIDE
+  if (merged)
+    hipLaunchKernelGGL(project_blocks_den_kernel, dim3((unsigned)((rows + kBlock - 1) / kBlock)), dim3(kBlock),
+                       0, s, parts, g.nparts, rows, den);
   return (int)hipGetLastError();
 }
 
@@ -384,15 +671,19 @@ static int launch_project_blocks(const unsigned char *x, const float *xs, const 
       hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || cus <= 0)
     return OT_E_BAD_ARG;
   const int nblocks = (D + kBlocksK - 1) / kBlocksK;
-  if (rows > 64 && nblocks <= 16) {
+  // (the wide kernel addresses a workgroup's logits with 32 bits)
+  if (rows > 64 && nblocks <= 16 && V < (1 << 21)) {
 #define OT_PROJECT(KB_, TILES_, COLS_, WAVES_)                                                              \
   return launch_project_blocks_kernel<T, KB_, TILES_, COLS_, WAVES_>(x, xs, w, ws, bias, rows, D, V, logits, \
                                                                      den, parts, cus, s)
-    if (nblocks == 1) OT_PROJECT(1, 2, 64, 2);
-    if (nblocks == 2) OT_PROJECT(2, 2, 64, 2);
-    if (nblocks == 3) OT_PROJECT(3, 2, 32, 2);
-    if (nblocks == 4) OT_PROJECT(4, 2, 32, 2);
+#define OT_PROJECT_WIDE(KB_, TILES_, WAVES_)                                                                         \
+  return launch_project_blocks_wide<T, KB_, TILES_, WAVES_>(x, xs, w, ws, bias, rows, D, V, logits, den, parts, cus, s)
+    if (nblocks == 1) OT_PROJECT_WIDE(1, 2, 2);
+    if (nblocks == 2) OT_PROJECT_WIDE(2, 2, 2);
+    if (nblocks == 3) OT_PROJECT_WIDE(3, 2, 2);
+    if (nblocks == 4) OT_PROJECT_WIDE(4, 2, 2);
     if (nblocks <= 8) OT_PROJECT(8, 2, 32, 1);
+#undef OT_PROJECT_WIDE
     OT_PROJECT(16, 1, 16, 1);
 #undef OT_PROJECT
   }
