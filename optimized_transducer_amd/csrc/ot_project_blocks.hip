@@ -32,7 +32,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 constexpr int kBlocksK = 128;      // elements per scale
 constexpr int kBlocksUnit = 16;    // D is a multiple of this: one 16-byte load
 constexpr int kSmallCols = 64;     // vocabulary entries of a workgroup of the small kernel
-constexpr int kWideCols = 32;      // vocabulary entries of a stage of the wide kernel
+// the wide kernel: vocabulary entries of a stage, tiles of 16 rows of a wave, rows of a workgroup
+constexpr int kWideCols = 64, kWideTiles = 2, kWideRows = kWavesPerBlock * kWideTiles * 16;
 constexpr int kPartCols = 16;      // least vocabulary entries behind one partial log-sum-exp
 
 // a running log-sum-exp as (largest value, sum of exp(value - largest))
@@ -339,254 +340,298 @@ __global__ __launch_bounds__(kBlock, WAVES_PER_SIMD) void project_blocks_kernel(
   }
 }
 
-// Many rows of up to KB blocks.  A workgroup of 4 waves owns 64 * TILES packed rows; a wave holds
-// its 16 * TILES rows of x, widened, in registers for the whole walk over the vocabulary, so x is
-// read and widened once.  The weight goes by in stages of 32 vocabulary entries (all of D, 8-bit)
-// through two LDS buffers: the next stage's global loads are issued at the start of a stage and
-// written in its last part, with one barrier per stage.  16-byte slots of LDS are XOR-swizzled by
-// their row against bank conflicts.
+// Many rows of up to KB blocks.  A workgroup of 4 waves owns 128 packed rows; a wave holds its 32
+// rows of x, widened, in registers for the whole walk over the vocabulary, so x is read and widened
+// once.  The weight goes by in stages of 64 vocabulary entries (all of D, 8-bit, 32 KB at D = 512),
+// loaded straight into one of two LDS buffers, with one barrier per stage.
 //
-// The walk advances in steps of 16 vocabulary entries x one block (4 * TILES matrix instructions);
-// the LDS read of a step's weight is issued one step ahead.  Nothing in a step branches: rows past
-// the end are dropped by the bounds of the store's buffer view, entries past the end have weight 0
-// and a starting value of -inf.
+// Loads and stores share one in-order counter: whoever waits for a load waits for every store
+// before it, and stores are what takes longest here.  The next stage's loads are issued at the
+// start of a stage, in front of its stores, and what is waited for at its end is all but the last
+// kStores operations: the loads, and the stores of the stage before, which have had a whole
+// stage's time to drain.
+//
+// The walk advances in steps of 16 vocabulary entries x one block (8 matrix instructions); the LDS
+// read of a step's weight is issued one step ahead.  Rows past the end are dropped by the bounds of
+// the store's buffer view, entries past the end have weight 0 and are set to -inf.
 //
 // Which entry of the vocabulary a row of the accumulator tile stands for is free: it is chosen so
 // that a lane ends up with 16 bytes of consecutive logits and four lanes with 64, from one group of
 // 16 entries for 4-byte logits and from two for 2-byte ones.
-//   ALIGNED: 4 logits start at a multiple of 4 bytes (else 2-byte logits are stored one by one)
+//   ALIGNED: 16 bytes of logits start at a multiple of 4 bytes (else 2-byte logits one by one)
 // Lane l holds bytes [64 q + 16 (l / 16), + 16) of a block of row l % 16 (q = 0, 1); the first 8
 // feed matrix instruction 2 q and the others 2 q + 1, in both operands alike.
-template <class T, int KB, int TILES, int WAVES_PER_SIMD, bool ALIGNED, bool DEN>
-__global__ __launch_bounds__(kBlock, WAVES_PER_SIMD) void project_blocks_wide_kernel(
-    const unsigned char *__restrict__ x, const float *__restrict__ xs, const unsigned char *__restrict__ w,
-    const float *__restrict__ ws, const float *__restrict__ bias, int64_t rows, int D, int V,
-    int stages_per_part, void *__restrict__ logits, float *__restrict__ den, LogSum *__restrict__ parts) {
-  constexpr int kCols = kWideCols;
-  constexpr int kSlots = KB * 8;                    // 16-byte slots of a row
-  constexpr int kPieces = kCols * kSlots / kBlock;  // of a stage per thread
-  constexpr int kLdsSlots = kCols * kSlots + 8 * (kCols / 8);  // of a stage, padded (see place())
-  constexpr unsigned kOut = sizeof(T) == 4 ? 4u : 2u;
-  constexpr int kGroup = 16 / (int)kOut;            // consecutive entries of a lane
-  constexpr int kSubs = kGroup / 4;                 // groups of 16 entries behind them
-  constexpr unsigned kNowhere = 0xffffffe0u;        // an offset that a store drops
-  static_assert(kPieces * kBlock == kCols * kSlots, "");
-  __shared__ __attribute__((aligned(16))) i32x4 s_w[2][kLdsSlots];
-  __shared__ __attribute__((aligned(16))) float s_bias[2][kCols];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int r = lane & 15, h = lane >> 4;
-  const int nblocks = (D + kBlocksK - 1) / kBlocksK;
-  const int stages = (V + kCols - 1) / kCols;
-  const int part = blockIdx.y;
-  const int stage0 = part * stages_per_part, stage1 = min(stages, stage0 + stages_per_part);
+template <class T, int KB, bool ALIGNED, bool DEN>
+struct WideProject {
+  static constexpr int kSlots = KB * 8;  // 16-byte slots of a row
+  static constexpr int kPieces = kWideCols * kSlots / kBlock;  // loads of a stage per thread
+  static constexpr unsigned kOut = sizeof(T) == 4 ? 4u : 2u;
+  static constexpr int kGroup = 16 / (int)kOut;  // consecutive entries of a lane
+  static constexpr int kSubs = kGroup / 4;       // groups of 16 entries behind them
+  static constexpr int kGroups = kWideCols / 16;
+  static constexpr int kStores = kGroups / kSubs * kWideTiles;  // of a stage, at least
+  typedef i32x4 Weights[kWideCols * kSlots];
+  typedef float Biases[kWideCols];
 
-  // Place of a 16-byte slot of a stage's row in LDS.  A 16-byte read is served 16 lanes at a time:
-  // lanes 0-7 and 24-31 of a half-wave, or 8-23, that is r < 8 of one h and r >= 8 of the other.
-  // Three bits of the row that lane r reads (r & 7) spread 8 lanes over 128 bytes; the other 8 are
-  // half of the 256 bytes that the banks hold away, by a pad of 128 bytes every 8 rows of r.
-  auto place = [&](int row, int slot) -> int {
-    const int lane8 = kSubs == 1 ? row & 7 : (row & 3) | ((row >> 1) & 4);
-    const int half = kSubs == 1 ? row >> 3 : row >> 4;
-    return row * kSlots + (KB % 2 == 0 ? 8 * half : 0) + (slot ^ lane8);
-  };
-  i32x4 piece[kPieces];
-  float piece_bias = 0.f;
-  auto load_stage = [&](int stage) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int p = tid + i * kBlock, row = p / kSlots, slot = p % kSlots;
-      const int v = stage * kCols + row;
-      piece[i] = i32x4{0, 0, 0, 0};
-      if (slot * 16 < D && v < V) piece[i] = *reinterpret_cast<const i32x4 *>(w + (int64_t)v * D + slot * 16);
-    }
-    if (tid < kCols) {
-      const int v = stage * kCols + tid;
-      piece_bias = v < V ? (bias ? bias[v] : 0.f) : OT_NEG_INF;
-    }
-  };
-  auto store_stage = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int p = tid + i * kBlock, row = p / kSlots, slot = p % kSlots;
-      s_w[buf][place(row, slot)] = piece[i];
-    }
-    if (tid < kCols) s_bias[buf][tid] = piece_bias;
-  };
-
-  load_stage(stage0);
-  const int64_t group0 = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * (64 * TILES);
-  if (group0 >= rows) return;
-  const int64_t row0 = group0 + wave * (16 * TILES);
-  bf16x8 xf[TILES][KB][4];
-  float xscale[TILES][KB];
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    const int64_t row = min(row0 + 16 * t + r, rows - 1);
-    const unsigned char *xr = x + row * D;
-#pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      xscale[t][b] = b < nblocks ? xs[row * nblocks + b] : 0.f;
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int k = b * kBlocksK + 64 * q + 16 * h;
-        i32x4 c = {0, 0, 0, 0};
-        if (k < D) c = *reinterpret_cast<const i32x4 *>(xr + k);
-        xf[t][b][2 * q] = widen(c[0], c[1]);
-        xf[t][b][2 * q + 1] = widen(c[2], c[3]);
-      }
-    }
-  }
-  store_stage(0);
-  lds_barrier();
-
-  // this workgroup's logits; a lane's byte offset of row t at its first entry of a stage
-  const __amdgpu_buffer_rsrc_t out =
-      make_buffer(static_cast<char *>(logits) + group0 * V * kOut,
-                  (unsigned)min((int64_t)(64 * TILES), rows - group0) * (unsigned)V * kOut);
-  const unsigned out_row = ((unsigned)(wave * (16 * TILES) + r) * (unsigned)V + (unsigned)(kGroup * h)) * kOut;
-  const unsigned out_tile = 16u * (unsigned)V * kOut;
-
-  // running log-sum-exp of this lane's share of its rows, relative to ref, which follows the
-  // largest value so far at a distance of at most 20
-  constexpr float kLog2e = 1.44269502162933349609375f;
-  float ref[TILES], sum[TILES];
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    ref[t] = -1e30f;
-    sum[t] = 0.f;
-  }
-
-  // Row m = 4 h + i of the tile of group `sub` stands for entry kGroup * h + 4 * sub + i of the
-  // 16 * kSubs entries.  As an operand row it is lane r = m.
-  const int entry0 = kGroup * (r >> 2) + (r & 3);
-  // slot 4 q + h of a block, swizzled by the entry's row in LDS: its low three bits
-  auto weight_at = [&](int sub, int q) -> const i32x4 * {
-    return &s_w[0][place(entry0 + 4 * sub, 4 * q + h)];
-  };
-  const i32x4 *read_at[kSubs][2];
-#pragma unroll
-  for (int sub = 0; sub < kSubs; ++sub)
-#pragma unroll
-    for (int q = 0; q < 2; ++q) read_at[sub][q] = weight_at(sub, q);
-  // step (group of 16 entries `g` of the stage, block b) of buffer buf
-  auto read_weight = [&](int buf, int g, int b, i32x4 (&f)[2]) {
-    const int at = buf * kLdsSlots + (kSubs == 1 && g == 1 ? place(16, 0) : 0) + 8 * b;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) f[q] = read_at[g % kSubs][q][at];
-  };
-
+  const unsigned char *w;
+  const float *ws, *bias;
+  int D, V, lane, wave, r, h;
+  bf16x8 x[kWideTiles][KB][4];
+  const float (*xs)[16][kWideTiles];  // this wave's scales of x in LDS
+  __amdgpu_buffer_rsrc_t out;
+  unsigned out_row, out_tile;  // byte offsets of this lane's first logit and from tile to tile
+  float ref[kWideTiles], sum[kWideTiles];
   i32x4 raw[2][2];  // weight of a step and of the next one
-  read_weight(0, 0, 0, raw[0]);
-  float scale[TILES][KB];
-  for (int stage = stage0; stage < stage1; ++stage) {
-    const int buf = (stage - stage0) & 1;
-    const bool more = stage + 1 < stage1;
-    if (more) load_stage(stage + 1);
-    {  // the stage lies in one block of 128 vocabulary entries
-      const float *wsr = ws + (int64_t)(stage * kCols / kBlocksK) * nblocks;
+  int at[kSubs][2][2];
+
+  // entry of a stage that row m of group g's tile stands for, as an operand row and as a result
+  __device__ __forceinline__ static int entry(int g, int m) {
+    return (g / kSubs) * (16 * kSubs) + kGroup * (m >> 2) + 4 * (g % kSubs) + (m & 3);
+  }
+  // A 16-byte read is served 16 lanes at a time: lanes 0-7 and 24-31 of a half-wave, or 8-23.
+  // Where rows are a multiple of 256 bytes, the number of the lane that reads a row (entry()
+  // backwards) spreads those over all 64 banks; with others, three bits of it and the rows' own
+  // offset do.
+  __device__ __forceinline__ static int swizzle(int row) {
+    const int m = kSubs == 1 ? row & 15 : (row & 3) | ((row >> 1) & 12);
+    return KB % 2 == 0 ? m : m & 7;
+  }
+
+  // the weight and the bias of a stage into LDS; entries past the end and elements past D are 0
+  __device__ __forceinline__ void load(int stage, i32x4 *weights, float *biases) const {
+    const int v0 = min(stage * kWideCols, V), n = min(kWideCols, V - v0);
+    const __amdgpu_buffer_rsrc_t from = make_buffer(w + (int64_t)min(v0, V - 1) * D, (unsigned)n * (unsigned)D);
 #pragma unroll
-      for (int c = 0; c < KB; ++c) {
-        const float sw = c < nblocks ? wsr[c] : 0.f;
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) scale[t][c] = xscale[t][c] * sw;
-      }
+    for (int i = 0; i < kPieces; ++i) {
+      const int first = (wave * kPieces + i) * kWave, p = first + lane;
+      const int row = p / kSlots, slot = (p % kSlots) ^ swizzle(row);
+      const unsigned src = slot * 16 < D ? (unsigned)row * (unsigned)D + 16u * slot : 0x7fffffffu;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)(weights + first), 16,
+                                               src, 0, 0, 0);
     }
+    if (wave == 0) {
+      const __amdgpu_buffer_rsrc_t b =
+          make_buffer(bias ? bias + min(v0, V - 1) : (const float *)w, bias ? (unsigned)n * 4u : 0u);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void *)biases, 4,
+                                               (unsigned)lane * 4u, 0, 0, 0);
+    }
+  }
+
+  // the weight of step (group g, block b)
+  __device__ __forceinline__ void read(const i32x4 *weights, int g, int b, i32x4 (&f)[2]) const {
 #pragma unroll
-    for (int set = 0; set < kCols / (16 * kSubs); ++set) {
-      f32x4 acc[kSubs][TILES];
+    for (int q = 0; q < 2; ++q)
+      f[q] = weights[at[g % kSubs][q][b & 1] + (g / kSubs) * (16 * kSubs) * kSlots + 8 * (b & ~1)];
+  }
+
+  // one stage: its weight and bias are in LDS, its first step in raw[0]; the next stage's, if there
+  // is one, go to `next` and raw[0] (nothing may be on its way to LDS when a workgroup ends)
+  __device__ __forceinline__ void run(int stage, bool more, const i32x4 *weights, const float *biases,
+                                      i32x4 *next_weights, float *next_biases) {
+    if (more) load(stage + 1, next_weights, next_biases);
+    __builtin_amdgcn_sched_barrier(0);  // no store of this stage in front of its loads
+    const int v0 = stage * kWideCols;
+    const float *wsr = ws + (int64_t)(v0 / kBlocksK) * KB;  // the stage lies in one block of 128 entries
+    float sw[KB];
+#pragma unroll
+    for (int b = 0; b < KB; ++b) sw[b] = wsr[b];
+#pragma unroll
+    for (int set = 0; set < kGroups / kSubs; ++set) {
+      f32x4 acc[kSubs][kWideTiles];
 #pragma unroll
       for (int sub = 0; sub < kSubs; ++sub) {
         const int g = set * kSubs + sub;
-        if (g == kCols / 16 - 1 && more) store_stage(buf ^ 1);
-        const f32x4 start =
-            *reinterpret_cast<const f32x4 *>(&s_bias[buf][16 * kSubs * set + kGroup * h + 4 * sub]);
+        const f32x4 start = *reinterpret_cast<const f32x4 *>(biases + entry(g, 4 * h));
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
           const int cur = (g * KB + b) & 1;  // (a stage has an even number of steps)
-          // the next step's weight; behind the last step of a stage lies the barrier
-          if (b + 1 < KB) read_weight(buf, g, b + 1, raw[cur ^ 1]);
-          else if (g + 1 < kCols / 16) read_weight(buf, g + 1, 0, raw[cur ^ 1]);
-          else {
-            lds_barrier();
-            read_weight(buf ^ 1, 0, 0, raw[cur ^ 1]);
-          }
-          f32x4 p[TILES];
+          if (b + 1 < KB) read(weights, g, b + 1, raw[cur ^ 1]);
+          else if (g + 1 < kGroups) read(weights, g + 1, 0, raw[cur ^ 1]);
+          float scale[kWideTiles];
+#pragma unroll
+          for (int t = 0; t < kWideTiles; ++t) scale[t] = xs[b][r][t] * sw[b];
+          f32x4 p[kWideTiles];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const i32x4 d = raw[cur][i / 2];
             const bf16x8 wf = i & 1 ? widen(d[2], d[3]) : widen(d[0], d[1]);
             const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int t = 0; t < TILES; ++t)
-              p[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xf[t][b][i], i == 0 ? zero : p[t], 0, 0, 0);
+            for (int t = 0; t < kWideTiles; ++t)
+              p[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, x[t][b][i], i == 0 ? zero : p[t], 0, 0, 0);
           }
 #pragma unroll
-          for (int t = 0; t < TILES; ++t)
+          for (int t = 0; t < kWideTiles; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              acc[sub][t][i] = __builtin_fmaf(p[t][i], scale[t][b], b == 0 ? start[i] : acc[sub][t][i]);
+              acc[sub][t][i] = __builtin_fmaf(p[t][i], scale[t], b == 0 ? start[i] : acc[sub][t][i]);
         }
       }
-      // rounding, store, log-sum-exp
-      const int v0 = stage * kCols + 16 * kSubs * set;  // this lane: entries v0 + kGroup * h, + kGroup
-      const int v = v0 + kGroup * h;
-      const unsigned at = v + kGroup <= V ? out_row + (unsigned)v0 * kOut : kNowhere;
+      finish(v0, set, acc);
+    }
+    if (more) {
+      // Every set of a stage that V does not cut has stored kWideTiles times: all but the last
+      // kStores operations are over (vmcnt; the other counters free).
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(0x0f70 | kStores);
+      lds_barrier();
+      read(next_weights, 0, 0, raw[0]);
+    }
+  }
+
+  // rounding, store and log-sum-exp of entries [v0 + 16 * kSubs * set, + 16 * kSubs)
+  __device__ __forceinline__ void finish(int v0, int set, f32x4 (&acc)[kSubs][kWideTiles]) {
+    const int v = v0 + entry(set * kSubs, 4 * h);  // of this lane: kGroup entries
+    const bool whole = v0 + 16 * kSubs * (set + 1) <= V;
+    if (!whole) {
 #pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        const unsigned to = at == kNowhere ? kNowhere : at + t * out_tile;
-        if constexpr (kOut == 4) {
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[0][t]), out, to, 0, 0);
-        } else {
-          unsigned short e[8];
+      for (int i = 0; i < kGroup; ++i)
+        if (v + i >= V)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] = from_float<T>(acc[i / 4][t][i % 4]);
-          if constexpr (ALIGNED) {
-            u32x4 four;
+          for (int t = 0; t < kWideTiles; ++t) acc[i / 4][t][i % 4] = OT_NEG_INF;
+    }
+    u32x4 four[kWideTiles];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) four[i] = (unsigned)e[2 * i] | ((unsigned)e[2 * i + 1] << 16);
-            __builtin_amdgcn_raw_buffer_store_b128(four, out, to, 0, 0);
-          } else {
+    for (int t = 0; t < kWideTiles; ++t) {
+      if constexpr (kOut == 4) {
+        four[t] = __builtin_bit_cast(u32x4, acc[0][t]);
+      } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) __builtin_amdgcn_raw_buffer_store_b16(e[i], out, to + 2 * i, 0, 0);
-          }
-        }
-      }
-      if (v0 + 16 * kSubs > V && v < V && v + kGroup > V) {  // the lane whose entries V cuts
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-          const int64_t row = row0 + 16 * t + r;
-#pragma unroll
-          for (int i = 0; i < kGroup - 1; ++i)
-            if (v + i < V && row < rows) store_logit<T>(logits, row * V + v + i, acc[i / 4][t][i % 4]);
-        }
-      }
-      if constexpr (DEN) {
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-          float top = acc[0][t][0];
-#pragma unroll
-          for (int i = 1; i < kGroup; ++i) top = fmaxf(top, acc[i / 4][t][i % 4]);
-          const float to = top > ref[t] + 20.f ? fminf(top, 3e38f) : ref[t];
-          float s = sum[t] * __builtin_amdgcn_exp2f((ref[t] - to) * kLog2e);
-          // (a difference first: in powers of 2 the rounding of a large `to` would be an exponent)
-#pragma unroll
-          for (int i = 0; i < kGroup; ++i) s += __builtin_amdgcn_exp2f((acc[i / 4][t][i % 4] - to) * kLog2e);
-          sum[t] = s;
-          ref[t] = to;
+        for (int i = 0; i < 4; ++i) {
+          // the float32 sum is rounded, whatever else becomes of it: a multiply-add that rounds
+          // straight to float16 gives other bits now and then
+          float lo = acc[i / 2][t][2 * (i & 1)], hi = acc[i / 2][t][2 * (i & 1) + 1];
+          asm("" : "+v"(lo), "+v"(hi));
+          four[t][i] = (unsigned)from_float<T>(lo) | ((unsigned)from_float<T>(hi) << 16);
         }
       }
     }
+    const unsigned dst = out_row + (unsigned)(v0 + 16 * kSubs * set) * kOut;
+    if (ALIGNED) {
+      // (a group that V cuts goes past the bounds of the view: it is stored below)
+      const unsigned to = whole || v + kGroup <= V ? dst : 0xfffffff0u - out_tile;
+#pragma unroll
+      for (int t = 0; t < kWideTiles; ++t) __builtin_amdgcn_raw_buffer_store_b128(four[t], out, to + t * out_tile, 0, 0);
+    }
+    if (!ALIGNED || !whole) {
+#pragma unroll
+      for (int t = 0; t < kWideTiles; ++t)
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i)
+          if (v + i < V && (!ALIGNED || v + kGroup > V)) {
+            if constexpr (kOut == 4)
+              __builtin_amdgcn_raw_buffer_store_b32(four[t][i], out, dst + t * out_tile + 4 * i, 0, 0);
+            else
+              __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(four[t][i / 2] >> (16 * (i & 1))), out,
+                                                    dst + t * out_tile + 2 * i, 0, 0);
+          }
+    }
+    if constexpr (DEN) {
+      // running log-sum-exp of this lane's share of its rows, relative to ref, which follows the
+      // largest value so far at a distance of at most 20
+      constexpr float kLog2e = 1.44269502162933349609375f;
+#pragma unroll
+      for (int t = 0; t < kWideTiles; ++t) {
+        float top = acc[0][t][0];
+#pragma unroll
+        for (int i = 1; i < kGroup; ++i) top = fmaxf(top, acc[i / 4][t][i % 4]);
+        const float to = top > ref[t] + 20.f ? fminf(top, 3e38f) : ref[t];
+        float s = sum[t] * __builtin_amdgcn_exp2f((ref[t] - to) * kLog2e);
+        // (a difference first: in powers of 2 the rounding of a large `to` would be an exponent)
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) s += __builtin_amdgcn_exp2f((acc[i / 4][t][i % 4] - to) * kLog2e);
+        sum[t] = s;
+        ref[t] = to;
+      }
+    }
+  }
+};
+
+template <class T, int KB, bool ALIGNED, bool DEN>
+__global__ __launch_bounds__(kBlock, 2) void project_blocks_wide_kernel(
+    const unsigned char *__restrict__ x, const float *__restrict__ xs, const unsigned char *__restrict__ w,
+    const float *__restrict__ ws, const float *__restrict__ bias, int64_t rows, int D, int V,
+    int stages_per_part, void *__restrict__ logits, float *__restrict__ den, LogSum *__restrict__ parts) {
+  typedef WideProject<T, KB, ALIGNED, DEN> P;
+  // two variables each, and not one array: the compiler then knows that the loads into one do not
+  // touch what is read from the other
+  __shared__ __attribute__((aligned(16))) typename P::Weights s_w0, s_w1;
+  __shared__ __attribute__((aligned(16))) typename P::Biases s_b0, s_b1;
+  // scales of x: those of a lane's two rows side by side
+  __shared__ __attribute__((aligned(16))) float s_xs[kWavesPerBlock][KB][16][kWideTiles];
+  const int tid = threadIdx.x;
+  const int64_t group0 = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * kWideRows;
+  if (group0 >= rows) return;
+  const int stages = (V + kWideCols - 1) / kWideCols;
+  const int part = blockIdx.y;
+  const int stage0 = part * stages_per_part, stage1 = min(stages, stage0 + stages_per_part);
+
+  P p;
+  p.w = w;
+  p.ws = ws;
+  p.bias = bias;
+  p.D = D;
+  p.V = V;
+  p.lane = tid & 63;
+  p.wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  p.r = p.lane & 15;
+  p.h = p.lane >> 4;
+  p.load(stage0, s_w0, s_b0);
+  const int64_t row0 = group0 + p.wave * (16 * kWideTiles);
+#pragma unroll
+  for (int t = 0; t < kWideTiles; ++t) {
+    const int64_t row = min(row0 + 16 * t + p.r, rows - 1);
+    const unsigned char *xr = x + row * D;
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      if (p.h == 0) s_xs[p.wave][b][p.r][t] = xs[row * KB + b];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int k = b * kBlocksK + 64 * q + 16 * p.h;
+        i32x4 c = {0, 0, 0, 0};
+        if (k < D) c = *reinterpret_cast<const i32x4 *>(xr + k);
+        p.x[t][b][2 * q] = widen(c[0], c[1]);
+        p.x[t][b][2 * q + 1] = widen(c[2], c[3]);
+      }
+    }
+    p.ref[t] = -1e30f;
+    p.sum[t] = 0.f;
+  }
+  p.xs = s_xs[p.wave];
+#pragma unroll
+  for (int sub = 0; sub < P::kSubs; ++sub)
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int odd = 0; odd < 2; ++odd) {
+        const int row = P::entry(sub, p.r);
+        p.at[sub][q][odd] = row * P::kSlots + ((8 * odd + 4 * q + p.h) ^ P::swizzle(row));
+      }
+  // this workgroup's logits; rows past the end are dropped by the view's bounds
+  p.out = make_buffer(static_cast<char *>(logits) + group0 * V * P::kOut,
+                      (unsigned)min((int64_t)kWideRows, rows - group0) * (unsigned)V * P::kOut);
+  p.out_row = ((unsigned)(p.wave * (16 * kWideTiles) + p.r) * (unsigned)V + (unsigned)(P::kGroup * p.h)) * P::kOut;
+  p.out_tile = 16u * (unsigned)V * P::kOut;
+
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // all loads; the other counters free
+  lds_barrier();
+  p.read(s_w0, 0, 0, p.raw[0]);
+  for (int stage = stage0;;) {
+    p.run(stage, stage + 1 < stage1, s_w0, s_b0, s_w1, s_b1);
+    if (++stage == stage1) break;
+    p.run(stage, stage + 1 < stage1, s_w1, s_b1, s_w0, s_b0);
+    if (++stage == stage1) break;
   }
   if constexpr (DEN) {
     // the four lanes of a row meet
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-      LogSum run = {ref[t], sum[t]};
+    for (int t = 0; t < kWideTiles; ++t) {
+      LogSum run = {p.ref[t], p.sum[t]};
 #pragma unroll
       for (int d = 16; d < 64; d *= 2)
         run = merge(run, {__shfl_xor(run.m, d, kWave), __shfl_xor(run.s, d, kWave)});
-      const int64_t row = row0 + 16 * t + r;
-      if (h == 0 && row < rows) {
+      const int64_t row = row0 + 16 * t + p.r;
+      if (p.h == 0 && row < rows) {
         if (parts) parts[(int64_t)part * rows + row] = run;
         else den[row] = logf(run.s) + (__builtin_isinf(run.m) ? 0.f : run.m);
       }
@@ -637,23 +682,25 @@ static int launch_project_blocks_kernel(const unsigned char *x, const float *xs,
   return (int)hipGetLastError();
 }
 
-template <class T, int KB, int TILES, int WAVES_PER_SIMD>
+template <class T, int KB>
 static int launch_project_blocks_wide(const unsigned char *x, const float *xs, const unsigned char *w,
                                       const float *ws, const float *bias, int64_t rows, int32_t D, int32_t V,
                                       void *logits, float *den, LogSum *parts, int cus, hipStream_t s) {
-  const ProjectGrid g((rows + 64 * TILES - 1) / (64 * TILES), (V + kWideCols - 1) / kWideCols,
-                      (int64_t)cus * WAVES_PER_SIMD);
+  const ProjectGrid g((rows + kWideRows - 1) / kWideRows, (V + kWideCols - 1) / kWideCols, 2 * (int64_t)cus);
   const bool merged = den && g.nparts > 1;
-#define OT_WIDE(ALIGNED_, DEN_)                                                                             \
-  hipLaunchKernelGGL((project_blocks_wide_kernel<T, KB, TILES, WAVES_PER_SIMD, ALIGNED_, DEN_>), g.grid, dim3(kBlock), 0, s, \
-                     x, xs, w, ws, bias, rows, D, V, g.stages_per_part, logits, merged ? nullptr : den,      \
-                     merged ? parts : nullptr)
+#define OT_WIDE(ALIGNED_)                                                                                 \
+  if (den)                                                                                                \
+    hipLaunchKernelGGL((project_blocks_wide_kernel<T, KB, ALIGNED_, true>), g.grid, dim3(kBlock), 0, \
+                       s, x, xs, w, ws, bias, rows, D, V, g.stages_per_part, logits,                      \
+                       merged ? nullptr : den, merged ? parts : nullptr);                                 \
+  else                                                                                                    \
+    hipLaunchKernelGGL((project_blocks_wide_kernel<T, KB, ALIGNED_, false>), g.grid, dim3(kBlock), 0, \
+                       s, x, xs, w, ws, bias, rows, D, V, g.stages_per_part, logits, (float *)nullptr,    \
+                       (LogSum *)nullptr)
   if (sizeof(T) == 4 || (V % 2 == 0 && (reinterpret_cast<uintptr_t>(logits) & 3) == 0)) {
-    if (den) OT_WIDE(true, true);
-    else OT_WIDE(true, false);
+    OT_WIDE(true);
   } else if constexpr (sizeof(T) != 4) {
-    if (den) OT_WIDE(false, true);
-    else OT_WIDE(false, false);
+    OT_WIDE(false);
   }
 #undef OT_WIDE
   if (merged)
@@ -676,12 +723,12 @@ static int launch_project_blocks(const unsigned char *x, const float *xs, const 
 #define OT_PROJECT(KB_, TILES_, COLS_, WAVES_)                                                              \
   return launch_project_blocks_kernel<T, KB_, TILES_, COLS_, WAVES_>(x, xs, w, ws, bias, rows, D, V, logits, \
                                                                      den, parts, cus, s)
-#define OT_PROJECT_WIDE(KB_, TILES_, WAVES_)                                                                         \
-  return launch_project_blocks_wide<T, KB_, TILES_, WAVES_>(x, xs, w, ws, bias, rows, D, V, logits, den, parts, cus, s)
-    if (nblocks == 1) OT_PROJECT_WIDE(1, 2, 2);
-    if (nblocks == 2) OT_PROJECT_WIDE(2, 2, 2);
-    if (nblocks == 3) OT_PROJECT_WIDE(3, 2, 2);
-    if (nblocks == 4) OT_PROJECT_WIDE(4, 2, 2);
+#define OT_PROJECT_WIDE(KB_)                                                                         \
+  return launch_project_blocks_wide<T, KB_>(x, xs, w, ws, bias, rows, D, V, logits, den, parts, cus, s)
+    if (nblocks == 1) OT_PROJECT_WIDE(1);
+    if (nblocks == 2) OT_PROJECT_WIDE(2);
+    if (nblocks == 3) OT_PROJECT_WIDE(3);
+    if (nblocks == 4) OT_PROJECT_WIDE(4);
     if (nblocks <= 8) OT_PROJECT(8, 2, 32, 1);
 #undef OT_PROJECT_WIDE
     OT_PROJECT(16, 1, 16, 1);
