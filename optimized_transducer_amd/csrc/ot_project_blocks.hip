@@ -34,6 +34,7 @@ constexpr int kBlocksUnit = 16;    // D is a multiple of this: one 16-byte load
 constexpr int kSmallCols = 64;     // vocabulary entries of a workgroup of the small kernel
 // the wide kernel: vocabulary entries of a stage, tiles of 16 rows of a wave, rows of a workgroup
 constexpr int kWideCols = 64, kWideTiles = 2, kWideRows = kWavesPerBlock * kWideTiles * 16;
+constexpr int kDeepCols = 128;     // the deep kernel: vocabulary entries of a workgroup
 constexpr int kPartCols = 16;      // least vocabulary entries behind one partial log-sum-exp
 
 // a running log-sum-exp as (largest value, sum of exp(value - largest))
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(kBlock) void project_blocks_small_kernel(
       if (threadIdx.x < 16 && row0 + threadIdx.x < rows) {
         LogSum t = s_part[0][threadIdx.x];
         for (int k = 1; k < kWavesPerBlock; ++k) t = merge(t, s_part[k][threadIdx.x]);
-        parts[part * rows + row0 + threadIdx.x] = t;
+        parts[(row0 + threadIdx.x) * col_tiles + part] = t;
       }
     }
   }
@@ -160,183 +161,6 @@ __device__ __forceinline__ void store_logits4(void *logits, int64_t i, const flo
     const u32x2 t = {(unsigned)from_float<T>(y[0]) | ((unsigned)from_float<T>(y[1]) << 16),
                      (unsigned)from_float<T>(y[2]) | ((unsigned)from_float<T>(y[3]) << 16)};
     *reinterpret_cast<unaligned *>(static_cast<unsigned short *>(logits) + i) = t;
-  }
-}
-
-// Many rows.  A workgroup of 4 waves owns 64 * TILES packed rows; a wave holds its 16 * TILES
-// rows of x, widened, in registers for the whole walk over the vocabulary, so x is read and
-// widened once.  The weight goes by in stages of COLS vocabulary entries (8-bit, all of D)
-// through two LDS buffers: the next stage's global loads are in flight while a stage is
-// multiplied, and are written to the other buffer behind it.  16-byte slots of LDS are
-// XOR-swizzled by their row against bank conflicts.
-//   KB: blocks of 128 in D that registers are laid out for (D may have fewer)
-// Lane l holds bytes [64 q + 16 (l / 16), + 16) of a block of row l % 16 (q = 0, 1); the first 8
-// feed matrix instruction 2 q and the others 2 q + 1, in both operands alike.
-template <class T, int KB, int TILES, int COLS, int WAVES_PER_SIMD>
-__global__ __launch_bounds__(kBlock, WAVES_PER_SIMD) void project_blocks_kernel(
-    const unsigned char *__restrict__ x, const float *__restrict__ xs, const unsigned char *__restrict__ w,
-    const float *__restrict__ ws, const float *__restrict__ bias, int64_t rows, int D, int V,
-    int stages_per_part, void *__restrict__ logits, float *__restrict__ den, LogSum *__restrict__ parts) {
-  constexpr int kRowBytes = KB * kBlocksK, kSlots = kRowBytes / 16;
-  constexpr int kPieces = COLS * kSlots / kBlock;  // 16-byte pieces of a stage per thread
-  static_assert(kPieces * kBlock == COLS * kSlots && COLS % 16 == 0 && kBlocksK % COLS == 0, "");
-  __shared__ __attribute__((aligned(16))) unsigned char s_w[2][COLS * kRowBytes];
-  __shared__ __attribute__((aligned(16))) float s_bias[2][COLS];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int r = lane & 15, h = lane >> 4;
-  const int nblocks = (D + kBlocksK - 1) / kBlocksK;
-  const int stages = (V + COLS - 1) / COLS;
-  const int part = blockIdx.y;
-  const int stage0 = part * stages_per_part, stage1 = min(stages, stage0 + stages_per_part);
-
-  // this thread's pieces of a stage: row, slot and place in LDS
-  i32x4 piece[kPieces];
-  float piece_bias;
-  auto load_stage = [&](int stage) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int p = tid + i * kBlock, row = p / kSlots, slot = p % kSlots;
-      const int v = min(stage * COLS + row, V - 1);  // entries past the end are masked later
-      piece[i] = i32x4{0, 0, 0, 0};
-      if (slot * 16 < D) piece[i] = *reinterpret_cast<const i32x4 *>(w + (int64_t)v * D + slot * 16);
-    }
-    if (tid < COLS) {
-      const int v = stage * COLS + tid;
-      piece_bias = v < V ? (bias ? bias[v] : 0.f) : OT_NEG_INF;
-    }
-  };
-  auto store_stage = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int p = tid + i * kBlock, row = p / kSlots, slot = p % kSlots;
-      *reinterpret_cast<i32x4 *>(&s_w[buf][row * kRowBytes + ((slot ^ (row & 7)) * 16)]) = piece[i];
-    }
-    if (tid < COLS) s_bias[buf][tid] = piece_bias;
-  };
-
-  load_stage(stage0);
-  // x: 16 * TILES rows per wave
-  const int64_t row0 = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * (64 * TILES) + wave * (16 * TILES);
-  bf16x8 xf[TILES][KB][4];
-  float xscale[TILES][KB];
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    const int64_t row = min(row0 + 16 * t + r, rows - 1);
-    const unsigned char *xr = x + row * D;
-#pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      xscale[t][b] = b < nblocks ? xs[row * nblocks + b] : 0.f;
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int k = b * kBlocksK + 64 * q + 16 * h;
-        i32x4 c = {0, 0, 0, 0};
-        if (k < D) c = *reinterpret_cast<const i32x4 *>(xr + k);
-        xf[t][b][2 * q] = widen(c[0], c[1]);
-        xf[t][b][2 * q + 1] = widen(c[2], c[3]);
-      }
-    }
-  }
-  store_stage(0);
-
-  // running log-sum-exp of this lane's share of its rows, relative to ref: ref follows the
-  // largest value so far at a distance of at most 20, so that few values make it move
-  float ref[TILES], sum[TILES];
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    ref[t] = OT_NEG_INF;
-    sum[t] = 0.f;
-  }
-  const bool want_den = den || parts;
-
-  for (int stage = stage0; stage < stage1; ++stage) {
-    const int buf = (stage - stage0) & 1;
-    lds_barrier();  // LDS only: the logits' stores stay in flight
-    if (stage + 1 < stage1) load_stage(stage + 1);
-    // the stage lies in one block of 128 vocabulary entries
-    const float *wsr = ws + (int64_t)(stage * COLS / kBlocksK) * nblocks;
-    float scale[TILES][KB];
-#pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      const float sw = b < nblocks ? wsr[b] : 0.f;
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) scale[t][b] = xscale[t][b] * sw;
-    }
-#pragma unroll 1
-    for (int c = 0; c < COLS / 16; ++c) {
-      const int v0 = stage * COLS + 16 * c;
-      if (v0 >= V) break;
-      const f32x4 b4 = *reinterpret_cast<const f32x4 *>(&s_bias[buf][16 * c + 4 * h]);
-      f32x4 acc[TILES];
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) acc[t] = b4;
-      const unsigned char *wr = &s_w[buf][(16 * c + r) * kRowBytes];
-#pragma unroll
-      for (int b = 0; b < KB; ++b) {
-        if (KB > 4 && b >= nblocks) continue;
-        f32x4 p[TILES];
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const i32x4 d = *reinterpret_cast<const i32x4 *>(wr + (((b * 8 + 4 * q + h) ^ (r & 7)) * 16));
-          const bf16x8 w0 = widen(d[0], d[1]), w1 = widen(d[2], d[3]);
-#pragma unroll
-          for (int t = 0; t < TILES; ++t)
-            p[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w0, xf[t][b][2 * q], p[t], 0, 0, 0);
-#pragma unroll
-          for (int t = 0; t < TILES; ++t)
-            p[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w1, xf[t][b][2 * q + 1], p[t], 0, 0, 0);
-        }
-#pragma unroll
-        for (int t = 0; t < TILES; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(p[t][i], scale[t][b], acc[t][i]);
-      }
-      // register i: vocabulary entry v0 + 4 h + i of row 16 t + r
-      const int v = v0 + 4 * h;
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        float y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = v0 + 16 <= V || v + i < V ? acc[t][i] : OT_NEG_INF;
-        const int64_t row = row0 + 16 * t + r;
-        if (row < rows) {
-          if (v + 4 <= V) {
-            store_logits4<T>(logits, row * V + v, y);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (v + i < V) store_logit<T>(logits, row * V + v + i, y[i]);
-          }
-        }
-        if (want_den) {
-          constexpr float kLog2e = 1.44269502162933349609375f;
-          const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
-          if (top > ref[t] + 20.f) {
-            if (sum[t] != 0.f) sum[t] *= expf(ref[t] - top);
-            ref[t] = top;
-          }
-          const float shift = __builtin_isinf(ref[t]) ? 0.f : -ref[t];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum[t] += __builtin_amdgcn_exp2f((y[i] + shift) * kLog2e);
-        }
-      }
-    }
-    if (stage + 1 < stage1) store_stage(buf ^ 1);
-  }
-  if (!want_den) return;
-  // the four lanes of a row meet
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    LogSum run = {ref[t], sum[t]};
-#pragma unroll
-    for (int d = 16; d < 64; d *= 2)
-      run = merge(run, {__shfl_xor(run.m, d, kWave), __shfl_xor(run.s, d, kWave)});
-    const int64_t row = row0 + 16 * t + r;
-    if (h == 0 && row < rows) {
-      if (parts) parts[(int64_t)part * rows + row] = run;
-      else den[row] = logf(run.s) + (__builtin_isinf(run.m) ? 0.f : run.m);
-    }
   }
 }
 
@@ -545,6 +369,23 @@ struct WideProject {
       }
     }
   }
+
+  // the four lanes of a row meet
+  __device__ __forceinline__ void finish_den(int64_t row0, int64_t rows, int part, int nparts, float *den,
+                                             LogSum *parts) const {
+#pragma unroll
+    for (int t = 0; t < kWideTiles; ++t) {
+      LogSum run = {ref[t], sum[t]};
+#pragma unroll
+      for (int d = 16; d < 64; d *= 2)
+        run = merge(run, {__shfl_xor(run.m, d, kWave), __shfl_xor(run.s, d, kWave)});
+      const int64_t row = row0 + 16 * t + r;
+      if (h == 0 && row < rows) {
+        if (parts) parts[row * nparts + part] = run;
+        else den[row] = logf(run.s) + (__builtin_isinf(run.m) ? 0.f : run.m);
+      }
+    }
+  }
 };
 
 template <class T, int KB, bool ALIGNED, bool DEN>
@@ -622,32 +463,183 @@ __global__ __launch_bounds__(kBlock, 2) void project_blocks_wide_kernel(
     p.run(stage, stage + 1 < stage1, s_w1, s_b1, s_w0, s_b0);
     if (++stage == stage1) break;
   }
-  if constexpr (DEN) {
-    // the four lanes of a row meet
-#pragma unroll
-    for (int t = 0; t < kWideTiles; ++t) {
-      LogSum run = {p.ref[t], p.sum[t]};
-#pragma unroll
-      for (int d = 16; d < 64; d *= 2)
-        run = merge(run, {__shfl_xor(run.m, d, kWave), __shfl_xor(run.s, d, kWave)});
-      const int64_t row = row0 + 16 * t + p.r;
-      if (p.h == 0 && row < rows) {
-        if (parts) parts[(int64_t)part * rows + row] = run;
-        else den[row] = logf(run.s) + (__builtin_isinf(run.m) ? 0.f : run.m);
-      }
-    }
-  }
+  if constexpr (DEN) p.finish_den(row0, rows, part, gridDim.y, den, parts);
 }
 
-// den[r] = log-sum-exp of a row's parts, merged in order
+// Many rows of any length.  A workgroup of 4 waves forms 128 packed rows x 128 vocabulary entries,
+// a wave 32 x 128 in 64 running sums per lane, block of D after block: the weight's block goes
+// straight into one of two LDS buffers, a wave's block of x into registers, both one step ahead of
+// the 64 matrix instructions of a step.  The workgroups of one group of rows have ids 8 apart and
+// run on one XCD, whose L2 serves x to all but the first.
+template <class T, bool ALIGNED, bool DEN>
+struct DeepProject {
+  typedef WideProject<T, 1, ALIGNED, DEN> Wide;  // one block: layout of a step, epilogue
+  static constexpr int kSubs = Wide::kSubs;
+  static constexpr int kGroups = kDeepCols / 16;
+  typedef i32x4 Weights[kDeepCols * 8];
+
+  Wide e;
+  const unsigned char *x[kWideTiles];  // this lane's rows
+  const float *xs[kWideTiles];
+  int v0, nblocks;
+  f32x4 acc[kGroups][kWideTiles];
+  i32x4 raw[kWideTiles][2];
+  float raw_scale[kWideTiles];
+
+  __device__ __forceinline__ void load(int b, i32x4 *weights) {
+    const int n = min(kDeepCols, e.V - v0);
+    const __amdgpu_buffer_rsrc_t from = make_buffer(e.w + (int64_t)v0 * e.D, (unsigned)n * (unsigned)e.D);
+#pragma unroll
+    for (int i = 0; i < kDeepCols * 8 / kBlock; ++i) {
+      const int first = (e.wave * (kDeepCols * 8 / kBlock) + i) * kWave, p = first + e.lane;
+      const int row = p / 8, k = b * kBlocksK + 16 * ((p % 8) ^ Wide::swizzle(row));
+      const unsigned src = k < e.D ? (unsigned)row * (unsigned)e.D + (unsigned)k : 0xfffffff0u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)(weights + first), 16,
+                                               src, 0, 0, 0);
+    }
+#pragma unroll
+    for (int t = 0; t < kWideTiles; ++t) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int k = b * kBlocksK + 64 * q + 16 * e.h;
+        raw[t][q] = i32x4{0, 0, 0, 0};
+        if (k < e.D) raw[t][q] = *reinterpret_cast<const i32x4 *>(x[t] + k);
+      }
+      raw_scale[t] = xs[t][b];
+    }
+  }
+
+  __device__ __forceinline__ void run(int b, const i32x4 *weights, i32x4 *next) {
+    const float sw = e.ws[(int64_t)(v0 / kBlocksK) * nblocks + b];
+    bf16x8 xw[kWideTiles][4];
+    float scale[kWideTiles];
+#pragma unroll
+    for (int t = 0; t < kWideTiles; ++t) {
+      scale[t] = raw_scale[t] * sw;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        xw[t][2 * q] = widen(raw[t][q][0], raw[t][q][1]);
+        xw[t][2 * q + 1] = widen(raw[t][q][2], raw[t][q][3]);
+      }
+    }
+    if (b + 1 < nblocks) load(b + 1, next);
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      i32x4 d[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) d[q] = weights[e.at[g % kSubs][q][0] + (g / kSubs) * (16 * kSubs) * 8];
+      f32x4 p[kWideTiles];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bf16x8 wf = i & 1 ? widen(d[i / 2][2], d[i / 2][3]) : widen(d[i / 2][0], d[i / 2][1]);
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < kWideTiles; ++t)
+          p[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xw[t][i], i == 0 ? zero : p[t], 0, 0, 0);
+      }
+#pragma unroll
+      for (int t = 0; t < kWideTiles; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[g][t][i] = __builtin_fmaf(p[t][i], scale[t], acc[g][t][i]);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // the next step's loads; the other counters free
+    lds_barrier();
+  }
+};
+
+template <class T, bool ALIGNED, bool DEN>
+__global__ __launch_bounds__(kBlock, 2) void project_blocks_deep_kernel(
+    const unsigned char *__restrict__ x, const float *__restrict__ xs, const unsigned char *__restrict__ w,
+    const float *__restrict__ ws, const float *__restrict__ bias, int64_t rows, int D, int V, int chunks,
+    void *__restrict__ logits, float *__restrict__ den, LogSum *__restrict__ parts) {
+  typedef DeepProject<T, ALIGNED, DEN> P;
+  typedef typename P::Wide E;
+  __shared__ __attribute__((aligned(16))) typename P::Weights s_w0, s_w1;
+  const int64_t id = (int64_t)blockIdx.z * gridDim.x + blockIdx.x;
+  const int64_t k = id >> 3;
+  const int64_t group0 = (k / chunks * 8 + (id & 7)) * kWideRows;
+  if (group0 >= rows) return;
+  const int chunk = (int)(k % chunks);
+  P p;
+  p.e.w = w;
+  p.e.ws = ws;
+  p.e.D = D;
+  p.e.V = V;
+  p.e.lane = threadIdx.x & 63;
+  p.e.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = p.e.r = p.e.lane & 15, h = p.e.h = p.e.lane >> 4;
+  p.v0 = chunk * kDeepCols;
+  p.nblocks = (D + kBlocksK - 1) / kBlocksK;
+  const int64_t row0 = group0 + p.e.wave * (16 * kWideTiles);
+#pragma unroll
+  for (int t = 0; t < kWideTiles; ++t) {
+    const int64_t row = min(row0 + 16 * t + r, rows - 1);
+    p.x[t] = x + row * D;
+    p.xs[t] = xs + row * p.nblocks;
+    p.e.ref[t] = -1e30f;
+    p.e.sum[t] = 0.f;
+  }
+  p.load(0, s_w0);
+  // sums start from the bias
+#pragma unroll
+  for (int g = 0; g < P::kGroups; ++g)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int v = p.v0 + E::entry(g, 4 * h + i);
+      const float b = bias && v < V ? bias[v] : 0.f;
+#pragma unroll
+      for (int t = 0; t < kWideTiles; ++t) p.acc[g][t][i] = b;
+    }
+#pragma unroll
+  for (int sub = 0; sub < P::kSubs; ++sub)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int row = E::entry(sub, r);
+      p.e.at[sub][q][0] = row * 8 + ((4 * q + h) ^ E::swizzle(row));
+    }
+  p.e.out = make_buffer(static_cast<char *>(logits) + group0 * V * E::kOut,
+                        (unsigned)min((int64_t)kWideRows, rows - group0) * (unsigned)V * E::kOut);
+  p.e.out_row = ((unsigned)(p.e.wave * (16 * kWideTiles) + r) * (unsigned)V + (unsigned)(E::kGroup * h)) * E::kOut;
+  p.e.out_tile = 16u * (unsigned)V * E::kOut;
+  __builtin_amdgcn_s_waitcnt(0x0f70);
+  lds_barrier();
+  for (int b = 0;;) {
+    p.run(b, s_w0, s_w1);
+    if (++b == p.nblocks) break;
+    p.run(b, s_w1, s_w0);
+    if (++b == p.nblocks) break;
+  }
+#pragma unroll
+  for (int set = 0; set < P::kGroups / P::kSubs; ++set) {
+    f32x4 a[P::kSubs][kWideTiles];
+#pragma unroll
+    for (int sub = 0; sub < P::kSubs; ++sub)
+#pragma unroll
+      for (int t = 0; t < kWideTiles; ++t) a[sub][t] = p.acc[set * P::kSubs + sub][t];
+    p.e.finish(p.v0, set, a);
+  }
+  if constexpr (DEN) p.e.finish_den(row0, rows, chunk, chunks, den, parts);
+}
+
+// den[r] = log-sum-exp of a row's parts: 16 lanes a row, merged in a fixed order
 __global__ __launch_bounds__(kBlock) void project_blocks_den_kernel(const LogSum *__restrict__ parts,
                                                                    int nparts, int64_t rows,
                                                                    float *__restrict__ den) {
-  const int64_t r = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  if (r >= rows) return;
-  LogSum t = parts[r];
-  for (int k = 1; k < nparts; ++k) t = merge(t, parts[(int64_t)k * rows + r]);
-  den[r] = logf(t.s) + (__builtin_isinf(t.m) ? 0.f : t.m);
+  for (int64_t r0 = (int64_t)blockIdx.x * (kBlock / 16); r0 < rows; r0 += (int64_t)gridDim.x * (kBlock / 16)) {
+    const int64_t r = r0 + threadIdx.x / 16;
+    LogSum t = {OT_NEG_INF, 0.f};
+    if (r < rows)
+      for (int k = threadIdx.x % 16; k < nparts; k += 16) t = merge(t, parts[r * nparts + k]);
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) t = merge(t, {__shfl_xor(t.m, d, kWave), __shfl_xor(t.s, d, kWave)});
+    if (threadIdx.x % 16 == 0 && r < rows) den[r] = logf(t.s) + (__builtin_isinf(t.m) ? 0.f : t.m);
+  }
+}
+
+static void launch_den(const LogSum *parts, int nparts, int64_t rows, float *den, hipStream_t s) {
+  const int64_t groups = (rows + kBlock / 16 - 1) / (kBlock / 16);
+  hipLaunchKernelGGL(project_blocks_den_kernel, dim3((unsigned)(groups < (1 << 20) ? groups : (1 << 20))),
+                     dim3(kBlock), 0, s, parts, nparts, rows, den);
 }
 
 // Workgroups of a launch: a part of the vocabulary for each where the rows alone do not fill the
@@ -666,21 +658,6 @@ struct ProjectGrid {
                 (unsigned)((row_groups + kMostX - 1) / kMostX));
   }
 };
-
-template <class T, int KB, int TILES, int COLS, int WAVES_PER_SIMD>
-static int launch_project_blocks_kernel(const unsigned char *x, const float *xs, const unsigned char *w,
-                                        const float *ws, const float *bias, int64_t rows, int32_t D, int32_t V,
-                                        void *logits, float *den, LogSum *parts, int cus, hipStream_t s) {
-  const ProjectGrid g((rows + 64 * TILES - 1) / (64 * TILES), (V + COLS - 1) / COLS, (int64_t)cus * WAVES_PER_SIMD);
-  const bool merged = den && g.nparts > 1;
-  hipLaunchKernelGGL((project_blocks_kernel<T, KB, TILES, COLS, WAVES_PER_SIMD>),
-                     g.grid, dim3(kBlock), 0, s, x, xs, w, ws, bias, rows, D, V, g.stages_per_part, logits,
-                     merged ? nullptr : den, merged ? parts : nullptr);
-  if (merged)
-    hipLaunchKernelGGL(project_blocks_den_kernel, dim3((unsigned)((rows + kBlock - 1) / kBlock)), dim3(kBlock),
-                       0, s, parts, g.nparts, rows, den);
-  return (int)hipGetLastError();
-}
 
 template <class T, int KB>
 static int launch_project_blocks_wide(const unsigned char *x, const float *xs, const unsigned char *w,
@@ -703,9 +680,34 @@ static int launch_project_blocks_wide(const unsigned char *x, const float *xs, c
     OT_WIDE(false);
   }
 #undef OT_WIDE
-  if (merged)
-    hipLaunchKernelGGL(project_blocks_den_kernel, dim3((unsigned)((rows + kBlock - 1) / kBlock)), dim3(kBlock),
-                       0, s, parts, g.nparts, rows, den);
+  if (merged) launch_den(parts, g.nparts, rows, den, s);
+  return (int)hipGetLastError();
+}
+
+template <class T>
+static int launch_project_blocks_deep(const unsigned char *x, const float *xs, const unsigned char *w,
+                                      const float *ws, const float *bias, int64_t rows, int32_t D, int32_t V,
+                                      void *logits, float *den, LogSum *parts, hipStream_t s) {
+  const int chunks = (V + kDeepCols - 1) / kDeepCols;
+  const int64_t row_groups = (rows + kWideRows - 1) / kWideRows, groups = (row_groups + 7) / 8 * 8 * chunks;
+  // (a launch holds 2^32 threads at most in each direction; a multiple of 8 keeps the ids' order)
+  constexpr int64_t kMostX = 1 << 20;
+  const dim3 grid((unsigned)(groups < kMostX ? groups : kMostX), 1, (unsigned)((groups + kMostX - 1) / kMostX));
+  const bool merged = den && chunks > 1;
+#define OT_DEEP(ALIGNED_)                                                                                     \
+  if (den)                                                                                                    \
+    hipLaunchKernelGGL((project_blocks_deep_kernel<T, ALIGNED_, true>), grid, dim3(kBlock), 0, s, x, xs, w, ws, \
+                       bias, rows, D, V, chunks, logits, merged ? nullptr : den, merged ? parts : nullptr);   \
+  else                                                                                                        \
+    hipLaunchKernelGGL((project_blocks_deep_kernel<T, ALIGNED_, false>), grid, dim3(kBlock), 0, s, x, xs, w,  \
+                       ws, bias, rows, D, V, chunks, logits, (float *)nullptr, (LogSum *)nullptr)
+  if (sizeof(T) == 4 || (V % 2 == 0 && (reinterpret_cast<uintptr_t>(logits) & 3) == 0)) {
+    OT_DEEP(true);
+  } else if constexpr (sizeof(T) != 4) {
+    OT_DEEP(false);
+  }
+#undef OT_DEEP
+  if (merged) launch_den(parts, chunks, rows, den, s);
   return (int)hipGetLastError();
 }
 
@@ -718,30 +720,23 @@ static int launch_project_blocks(const unsigned char *x, const float *xs, const 
       hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || cus <= 0)
     return OT_E_BAD_ARG;
   const int nblocks = (D + kBlocksK - 1) / kBlocksK;
-  // (the wide kernel addresses a workgroup's logits with 32 bits)
-  if (rows > 64 && nblocks <= 16 && V < (1 << 21)) {
-#define OT_PROJECT(KB_, TILES_, COLS_, WAVES_)                                                              \
-  return launch_project_blocks_kernel<T, KB_, TILES_, COLS_, WAVES_>(x, xs, w, ws, bias, rows, D, V, logits, \
-                                                                     den, parts, cus, s)
-#define OT_PROJECT_WIDE(KB_)                                                                         \
+  // (both kernels address a workgroup's logits, and the deep one its weights, with 32 bits)
+  if (rows > 64 && V < (1 << 21) && D < (1 << 24)) {
+#define OT_PROJECT_WIDE(KB_) \
   return launch_project_blocks_wide<T, KB_>(x, xs, w, ws, bias, rows, D, V, logits, den, parts, cus, s)
     if (nblocks == 1) OT_PROJECT_WIDE(1);
     if (nblocks == 2) OT_PROJECT_WIDE(2);
     if (nblocks == 3) OT_PROJECT_WIDE(3);
     if (nblocks == 4) OT_PROJECT_WIDE(4);
-    if (nblocks <= 8) OT_PROJECT(8, 2, 32, 1);
 #undef OT_PROJECT_WIDE
-    OT_PROJECT(16, 1, 16, 1);
-#undef OT_PROJECT
+    return launch_project_blocks_deep<T>(x, xs, w, ws, bias, rows, D, V, logits, den, parts, s);
   }
   const int col_tiles = (V + kSmallCols - 1) / kSmallCols;
   const int64_t tiles = (rows + 15) / 16 * col_tiles;
   const dim3 grid((unsigned)(tiles < (1 << 22) ? tiles : (1 << 22)));
   hipLaunchKernelGGL((project_blocks_small_kernel<T>), grid, dim3(kBlock), 0, s, x, xs, w, ws, bias, rows, D,
                      V, col_tiles, tiles, logits, den ? parts : nullptr);
-  if (den)
-    hipLaunchKernelGGL(project_blocks_den_kernel, dim3((unsigned)((rows + kBlock - 1) / kBlock)), dim3(kBlock),
-                       0, s, parts, col_tiles, rows, den);
+  if (den) launch_den(parts, col_tiles, rows, den, s);
   return (int)hipGetLastError();
 }
 
