@@ -720,8 +720,18 @@ static int launch_project_blocks(const unsigned char *x, const float *xs, const 
       hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || cus <= 0)
     return OT_E_BAD_ARG;
   const int nblocks = (D + kBlocksK - 1) / kBlocksK;
-  // (both kernels address a workgroup's logits, and the deep one its weights, with 32 bits)
-  if (rows > 64 && V < (1 << 21) && D < (1 << 24)) {
+  const int col_tiles = (V + kSmallCols - 1) / kSmallCols;
+  const int64_t tiles = (rows + 15) / 16 * col_tiles;
+  // The small kernel spreads over the chip what the others would do on a few compute units, but
+  // reads its operands again for every 16 x 64 logits.  Microseconds with denominators, small
+  // against wide or deep, by its workgroups (256 compute units):
+  //   D = 512:  32 x 5000 (158) 10 : 12, 64 x 5000 (316) 12 : 12, 512 x 500 (256) 9 : 11,
+  //             1024 x 500 (512) 12 : 11, 128 x 5000 (632) 15 : 13
+  //   D = 1008: 256 x 5000 (1264) 26 : 31, 512 x 5000 (2528) 44 : 31
+  //   D = 2048: 512 x 500 (256) 16 : 32, 1024 x 500 (512) 26 : 32, 4096 x 500 (2048) 88 : 33
+  const bool few = nblocks <= 4 ? 2 * tiles <= 3 * (int64_t)cus : tiles * nblocks <= 40 * (int64_t)cus;
+  // (wide and deep address a workgroup's logits, and deep its weights, with 32 bits)
+  if (!few && V < (1 << 21) && D < (1 << 24)) {
 #define OT_PROJECT_WIDE(KB_) \
   return launch_project_blocks_wide<T, KB_>(x, xs, w, ws, bias, rows, D, V, logits, den, parts, cus, s)
     if (nblocks == 1) OT_PROJECT_WIDE(1);
@@ -731,8 +741,6 @@ static int launch_project_blocks(const unsigned char *x, const float *xs, const 
 #undef OT_PROJECT_WIDE
     return launch_project_blocks_deep<T>(x, xs, w, ws, bias, rows, D, V, logits, den, parts, s);
   }
-  const int col_tiles = (V + kSmallCols - 1) / kSmallCols;
-  const int64_t tiles = (rows + 15) / 16 * col_tiles;
   const dim3 grid((unsigned)(tiles < (1 << 22) ? tiles : (1 << 22)));
   hipLaunchKernelGGL((project_blocks_small_kernel<T>), grid, dim3(kBlock), 0, s, x, xs, w, ws, bias, rows, D,
                      V, col_tiles, tiles, logits, den ? parts : nullptr);

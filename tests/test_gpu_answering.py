@@ -135,7 +135,11 @@ def _check_project(args, host, dtype, denominators=True):
 SHAPES = [(1, 16, 1), (1, 128, 64), (2, 144, 5), (15, 64, 17), (16, 512, 500), (17, 512, 500), (32, 512, 500),
           (33, 1008, 131), (64, 256, 128), (65, 256, 129), (127, 128, 255), (128, 384, 256), (129, 640, 257),
           (1, 1024, 4096), (7, 2048, 1111), (300, 512, 500), (513, 192, 1030), (1003, 1008, 777), (2000, 512, 512),
-          (1, 4096, 33), (257, 80, 4999), (4100, 112, 96)]
+          (1, 4096, 33), (257, 80, 4999), (4100, 112, 96),
+          # each kernel at its smallest and odd sizes: blocks 1 to 4, then longer rows
+          (13000, 16, 33), (13000, 128, 65), (6600, 240, 127), (3300, 256, 250), (3301, 384, 251), (3333, 400, 129),
+          (1700, 512, 1021), (1700, 496, 1022), (6500, 1040, 257), (2111, 640, 1001), (5000, 2064, 130),
+          (700, 1536 + 16, 3001)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
