@@ -42,6 +42,8 @@ struct SampleSettings {
 };
 
 constexpr int kSampleBins = 256;
+constexpr int kSampleFew = 512;  // entries that one wave takes over from the others
+constexpr int64_t kAheadGroups = 256 * 7;  // workgroups of 4 rows
 constexpr float kInf = __builtin_huge_valf();
 
 // ---- wave-wide helpers ----------------------------------------------------------------------
@@ -87,8 +89,7 @@ __device__ __forceinline__ int wave_sum(int v) { return lane_value(wave_scan(v),
 
 template <int WAVES>
 struct SampleShared {
-  double bin_weight[kSampleBins];
-  unsigned bin_count[kSampleBins];
+  unsigned bins[kSampleBins];
   double sum[WAVES];
   float value[2][WAVES];
   int count[WAVES];
@@ -131,13 +132,17 @@ struct RowGroup {
   }
   // totals of a sum and a count, the same bits in every thread
   __device__ __forceinline__ void totals(double &sum, int &count) const {
-    sum = wave_sum(sum);
-    count = wave_sum(count);
+    gather(wave_sum(sum), wave_sum(count), sum, count);
+  }
+  // the same from every wave's part
+  __device__ __forceinline__ void gather(double part, int part_count, double &sum, int &count) const {
+    sum = part;
+    count = part_count;
     if constexpr (WAVES > 1) {
       sync();
       if (lane == 0) {
-        s.sum[wave] = sum;
-        s.count[wave] = count;
+        s.sum[wave] = part;
+        s.count[wave] = part_count;
       }
       sync();
       sum = 0.0;
@@ -242,6 +247,10 @@ struct Sampler {
   float floor_ = OT_NEG_INF;
   int floor_last = 0x7fffffff;
   double least = 0.0;
+  // sum of the remaining weights of this wave's part, where it is known, and entries at a value
+  double part = 0.0;
+  int part_at = 0;
+  bool part_known = false;
 
   __device__ __forceinline__ Sampler(const RowGroup<WAVES> &g_, const void *row_, int V_, int per_wave_, float m_,
                                      float temperature, float (&x_)[kHeld ? CHUNKS : 1][VEC])
@@ -334,17 +343,18 @@ struct Sampler {
   }
 
   // The largest value v such that the entries at or above it (their number, or with WEIGHTS
-  // their weights) reach `want`; by_above: what the entries above v come to.  With weights this
-  // goes by sums in whatever order the bins were filled: close, and for the caller to check.
+  // their weights) reach `want`, among those of [lo, m]; above: what the entries above v come to.
+  // With WEIGHTS this goes by 32-bit weights in whatever order the bins are filled: close, and
+  // for the caller to settle.  Without, it is content with a smaller value as soon as no more than
+  // `enough` entries are at or above it; above is then -1.
   template <bool WEIGHTS>
-  __device__ __forceinline__ float select(double want, float lo, double &above) {
+  __device__ __forceinline__ float select(double want, float lo, double &above, int enough = 0) {
+    float *const bin_weight = reinterpret_cast<float *>(g.s.bins);
     float hi = m;
     above = 0.0;
+    const float per_octave = (float)weight.c;
     while (lo < hi) {
-      for (int i = g.thread(); i < kSampleBins; i += WAVES * kWave) {
-        g.s.bin_count[i] = 0;
-        if (WEIGHTS) g.s.bin_weight[i] = 0.0;
-      }
+      for (int i = g.thread(); i < kSampleBins; i += WAVES * kWave) g.s.bins[i] = 0;  // (also as a float)
       g.sync();
       // bins of equal width; where that is no normal number, bins of the values' bit patterns.
       // Either way hi falls into the first bin and lo into the last.
@@ -357,47 +367,46 @@ struct Sampler {
         return by_value ? (int)fminf((hi - y) * per_unit, kSampleBins - 1.0f)
                         : (int)((hi_key - order_key(y)) >> shift);
       };
-      each([&](int j, int, const float *y) {
+      each([&](int, int, const float *y) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
           if (y[e] >= lo && y[e] <= hi) {
             const int b = bin(y[e]);
-            atomicAdd(&g.s.bin_count[b], 1u);
-            if (WEIGHTS) unsafeAtomicAdd(&g.s.bin_weight[b], weight_of(j, e, y[e]));
+            if constexpr (WEIGHTS) unsafeAtomicAdd(&bin_weight[b], __builtin_amdgcn_exp2f((y[e] - m) * per_octave));
+            else atomicAdd(&g.s.bins[b], 1u);
           }
       });
       g.sync();
       // every wave looks for the bin: lane l holds bins [4 l, 4 l + 4)
       constexpr int kPer = kSampleBins / kWave;
-      unsigned n[kPer];
       double amount[kPer], mine = 0.0;
 #pragma unroll
       for (int q = 0; q < kPer; ++q) {
-        const int b = g.lane * kPer + q;
-        n[q] = g.s.bin_count[b];
-        amount[q] = WEIGHTS ? g.s.bin_weight[b] : (double)n[q];
+        amount[q] = WEIGHTS ? (double)bin_weight[g.lane * kPer + q] : (double)g.s.bins[g.lane * kPer + q];
         mine += amount[q];
       }
       double run = above + (wave_scan(mine) - mine);
       int reached = kSampleBins, filled = -1;
-      double before_reached = 0.0, before_filled = 0.0;
+      double before_reached = 0.0, before_filled = 0.0, with_reached = 0.0;
 #pragma unroll
       for (int q = 0; q < kPer; ++q) {
-        if (n[q] > 0) {
+        if (amount[q] > 0.0) {
           filled = g.lane * kPer + q;
           before_filled = run;
           if (reached == kSampleBins && run + amount[q] >= want) {
             reached = filled;
             before_reached = run;
+            with_reached = run + amount[q];
           }
         }
         run += amount[q];
       }
       const uint64_t r = __ballot(reached < kSampleBins), f = __ballot(filled >= 0);
-      // (rounding alone can keep the last bin from reaching `want`)
-      const int src = r ? __builtin_ctzll(r) : 63 - __builtin_clzll(f);
-      const int pick = r ? lane_value(reached, src) : lane_value(filled, src);
-      above = r ? lane_value(before_reached, src) : lane_value(before_filled, src);
+      // (rounding can keep the last bin from reaching `want`, and all weights can be 0)
+      const int src = r ? __builtin_ctzll(r) : f ? 63 - __builtin_clzll(f) : 0;
+      const int pick = r ? lane_value(reached, src) : f ? lane_value(filled, src) : kSampleBins - 1;
+      above = r ? lane_value(before_reached, src) : f ? lane_value(before_filled, src) : above;
+      const bool content = !WEIGHTS && r && lane_value(with_reached, src) <= enough;
       float b_hi = OT_NEG_INF, b_lo = kInf;
       each([&](int, int, const float *y) {
 #pragma unroll
@@ -409,36 +418,76 @@ struct Sampler {
       });
       g.sync();  // the bins have been read
       g.extremes(b_hi, b_lo);
+      if (!(b_lo <= b_hi)) return hi;  // nothing there (no such entries or weights)
+      if (content) {
+        above = -1.0;
+        return b_lo;
+      }
       hi = b_hi;
       lo = b_lo;
     }
     return lo;
   }
 
-  // the smallest entry that is not excluded
-  __device__ __forceinline__ float smallest() {
-    float hi = OT_NEG_INF, lo = kInf;
+  // Copies the entries that can be among the first k of the order, kSampleFew at most, and their
+  // indices, in index order; k <= kSampleFew.  Returns their number.
+  __device__ __forceinline__ int gather_few(int k, float lowest, int finite, float *few, int *few_index) {
+    float v = lowest;
+    if (finite > kSampleFew) {
+      double above;
+      v = select<false>((double)k, lowest, above, kSampleFew);
+      if (above >= 0.0) {  // too many entries at v: only the first of them
+        int at_v = 0;
+        each([&](int, int, const float *y) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) at_v += y[e] == v;
+        });
+        double none = 0.0;
+        g.totals(none, at_v);
+        exclude(v, k - (int)above, at_v);
+      }
+    }
+    int here = 0;
     each([&](int, int, const float *y) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) here += __popcll(__ballot(y[e] >= v));
+    });
+    int at = 0, total = here;
+    if constexpr (WAVES > 1) {
+      g.sync();
+      if (g.lane == 0) g.s.count[g.wave] = here;
+      g.sync();
+      total = 0;
+      for (int q = 0; q < WAVES; ++q) {
+        if (q == g.wave) at = total;
+        total += g.s.count[q];
+      }
+    }
+    each([&](int, int i, const float *y) {
+      int to = at;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {  // entries of the lanes before
+        const uint64_t kept = __ballot(y[e] >= v);
+        to += __builtin_amdgcn_mbcnt_hi((unsigned)(kept >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)kept, 0));
+        at += __popcll(kept);
+      }
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
-        if (y[e] > OT_NEG_INF) lo = fminf(lo, y[e]);
+        if (y[e] >= v) {
+          few[to] = y[e];
+          few_index[to] = i + e;
+          ++to;
+        }
     });
-    g.extremes(hi, lo);
-    return lo;
+    g.sync();
+    return total;
   }
 
-  __device__ __forceinline__ void keep_top_k(int k) {
-    const float lo = smallest();
-    double finite = 0.0;
-    int count = 0;
-    each([&](int, int, const float *y) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) count += y[e] > OT_NEG_INF;
-    });
-    g.totals(finite, count);
-    if (k >= count) return;
+  // `lowest`: the smallest finite entry, `finite`: how many there are
+  __device__ __forceinline__ void keep_top_k(int k, float &lowest, int finite) {
+    if (k >= finite) return;
     double above;
-    const float v = select<false>((double)k, lo, above);
+    const float v = select<false>((double)k, lowest, above);
     int at_v = 0;
     each([&](int, int, const float *y) {
 #pragma unroll
@@ -447,34 +496,63 @@ struct Sampler {
     double none = 0.0;
     g.totals(none, at_v);
     exclude(v, k - (int)above, at_v);
+    lowest = v;
   }
 
-  // sum of the weights above v, and the number of entries at it
+  // Weights above v (those at or above it with `and_at`) and the number of entries at v: of this
+  // wave's part in part and part_at, of the row in sum and at_v.
+  template <bool AND_AT>
   __device__ __forceinline__ void sum_above(float v, double &sum, int &at_v) {
-    sum = 0.0;
-    at_v = 0;
+    part = 0.0;
+    part_at = 0;
     each([&](int j, int, const float *y) {
       double t[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        t[e] = y[e] > v ? weight_of(j, e, y[e]) : 0.0;
-        at_v += y[e] == v;
+        t[e] = y[e] > v || (AND_AT && y[e] == v) ? weight_of(j, e, y[e]) : 0.0;
+        part_at += y[e] == v;
       }
-      sum += pairwise(t);
+      part += pairwise(t);
     });
-    g.totals(sum, at_v);
+    part = wave_sum(part);
+    part_at = wave_sum(part_at);
+    g.gather(part, part_at, sum, at_v);
   }
 
-  __device__ __forceinline__ void keep_top_p(float p) {
+  __device__ __forceinline__ void keep_top_p(float p, float lowest) {
     double total;
     int none;
-    sum_above(OT_NEG_INF, total, none);
+    sum_above<true>(lowest, total, none);
     const double want = (double)p * total;
-    double above, sum;
-    const float v = select<true>(want, smallest(), above);
-    int at_v;
-    sum_above(v, sum, at_v);
-    const double wv = weight(v);
+    // Entries of weights below (1 - p) * total / V come to less than what lies behind the cut.
+    float from = lowest;
+    const double least_weight = (1.0 - (double)p) * total / V * 0.99;
+    if (least_weight > 1e-30) {
+      const float z = __log2f((float)least_weight) / (float)weight.c;
+      if (z > -1e30f) from = fminf(m, fmaxf(from, m + 1.001f * z));
+    }
+    double rough, sum;
+    float v = select<true>(want, from, rough);
+    int at_v, went = 0;
+    double wv;
+    for (;;) {
+      sum_above<false>(v, sum, at_v);
+      wv = weight(v);
+      // where the entries above v reach `want` already, or those at it do not: the next value
+      const int go = sum >= want && v < m ? 1 : sum + at_v * wv < want && v > lowest ? -1 : 0;
+      if (go == 0 || go == -went) break;  // (back and forth: the border lies within a rounding)
+      went = go;
+      float up = kInf, down = OT_NEG_INF;
+      each([&](int, int, const float *y) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          if (y[e] > v) up = fminf(up, y[e]);
+          if (y[e] < v) down = fmaxf(down, y[e]);
+        }
+      });
+      g.extremes(down, up);
+      v = go > 0 ? up : down;
+    }
     // of the entries at v, number j (from 0) remains if sum + j * wv < want
     int n = at_v;
     if (wv > 0.0) {
@@ -483,10 +561,21 @@ struct Sampler {
     }
     if (v == m) n = max(n, 1);
     exclude(v, n, at_v);
+    // this wave's part of what remains
+    int before = 0;
+    if constexpr (WAVES > 1) {
+      g.sync();
+      if (g.lane == 0) g.s.count[g.wave] = part_at;
+      g.sync();
+      for (int k = 0; k < g.wave; ++k) before += g.s.count[k];
+    }
+    part += max(0, min(n - before, part_at)) * wv;
+    part_known = true;
   }
 
   __device__ __forceinline__ void keep_min_p(float p) {
     least = p;
+    part_known = false;
     if constexpr (kHeldWeights) {
 #pragma unroll
       for (int j = 0; j < CHUNKS; ++j)
@@ -496,27 +585,35 @@ struct Sampler {
     }
   }
 
-  __device__ __forceinline__ Drawn draw(double u, int top_k, float top_p, float min_p) {
-    if (top_k > 0 && top_k < V) keep_top_k(top_k);
+  // the cuts; before them `lowest` is the smallest finite entry, of `finite` ones
+  __device__ __forceinline__ void cut(int top_k, float top_p, float min_p, float lowest, int finite) {
+    if (top_k > 0 && top_k < V) keep_top_k(top_k, lowest, finite);
+    weigh();
+    if (top_p < 1.f) keep_top_p(fmaxf(top_p, 0.f), lowest);
+    if (min_p > 0.f) keep_min_p(fminf(min_p, 1.f));
+  }
+  __device__ __forceinline__ void weigh() {
     if constexpr (kHeldWeights) {
 #pragma unroll
       for (int j = 0; j < CHUNKS; ++j)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) w[j][e] = weight(x[j][e]);
     }
-    if (top_p < 1.f) keep_top_p(top_p);
-    if (min_p > 0.f) keep_min_p(fminf(min_p, 1.f));
+  }
 
+  __device__ __forceinline__ Drawn draw(double u) {
     // totals of the waves' parts, then the part, the chunk, the lane and the element in which
     // the running sum passes u * total
-    double part = 0.0;
-    each([&](int j, int, const float *y) {
-      double t[VEC];
+    if (!part_known) {
+      part = 0.0;
+      each([&](int j, int, const float *y) {
+        double t[VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) t[e] = weight_of(j, e, y[e]);
-      part += pairwise(t);
-    });
-    part = wave_sum(part);
+        for (int e = 0; e < VEC; ++e) t[e] = weight_of(j, e, y[e]);
+        part += pairwise(t);
+      });
+      part = wave_sum(part);
+    }
     double total = part, before = 0.0;
     if constexpr (WAVES > 1) {
       g.sync();
@@ -615,61 +712,73 @@ struct Sampler {
   }
 };
 
-// One row: reads it, settles the rows without an answer and the greedy ones, draws from the
-// others.
-template <class T, int WAVES, int CHUNKS>
+// One row, in x if it is held: settles the rows without an answer and the greedy ones, draws from
+// the others.  FILTER: one of top_k, top_p and min_p may be in force.  Where top_k leaves few
+// entries of a row of several waves, one wave goes on with them alone.
+template <class T, int WAVES, int CHUNKS, bool FILTER>
 __device__ __forceinline__ void sample_row(const RowGroup<WAVES> &g, const void *row, int V, double u,
                                            float temperature, int top_k, float top_p, float min_p,
-                                           int32_t *symbol, float *log_prob) {
+                                           float (&x)[CHUNKS > 0 ? CHUNKS : 1][kSampleVec<T>], int32_t *symbol,
+                                           float *log_prob) {
   constexpr int VEC = kSampleVec<T>;
   constexpr bool kHeld = CHUNKS > 0;
   const int chunks = kHeld ? CHUNKS : (V + WAVES * kWave * VEC - 1) / (WAVES * kWave * VEC);
-  float x[kHeld ? CHUNKS : 1][VEC];
   auto first_index = [&](int j) { return ((g.wave * chunks + j) * kWave + g.lane) * VEC; };
-  float m = OT_NEG_INF, bad = 0.f;
-  auto look = [&](const float *y) {
+  auto each = [&](auto f) {
+    if constexpr (kHeld) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      m = fmaxf(m, y[e]);
-      if (y[e] != y[e]) bad = -1.f;
+      for (int j = 0; j < CHUNKS; ++j) f(j, x[j]);
+    } else {
+      for (int j = 0; j < chunks; ++j) {
+        float y[VEC];
+        load_logits<T>(row, first_index(j), V, y);
+        f(j, y);
+      }
     }
   };
-  if constexpr (kHeld) {
+  const bool cuts = FILTER && temperature > 0.f && ((top_k > 0 && top_k < V) || top_p < 1.f);
+  float m = OT_NEG_INF, bad = 0.f, lowest = kInf;
+  int finite = 0;
+  if (cuts) {
+    each([&](int, const float *y) {
 #pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) load_logits<T>(row, first_index(j), V, x[j]);
-#pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) look(x[j]);
+      for (int e = 0; e < VEC; ++e) {
+        m = fmaxf(m, y[e]);
+        if (y[e] != y[e]) bad = -1.f;
+        if (y[e] > OT_NEG_INF) {
+          lowest = fminf(lowest, y[e]);
+          ++finite;
+        }
+      }
+    });
+    float none = 0.f;
+    double nothing = 0.0;
+    g.extremes(none, bad);
+    g.extremes(m, lowest);
+    g.totals(nothing, finite);
   } else {
-    for (int j = 0; j < chunks; ++j) {
-      float y[VEC];
-      load_logits<T>(row, first_index(j), V, y);
-      look(y);
-    }
+    each([&](int, const float *y) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        m = fmaxf(m, y[e]);
+        if (y[e] != y[e]) bad = -1.f;
+      }
+    });
+    g.extremes(m, bad);
   }
-  g.extremes(m, bad);
   Drawn d = {-1, OT_NEG_INF};
   if (bad < 0.f || __builtin_isinf(m) || u != u) {
     // no answer
   } else if (!(temperature > 0.f)) {
     int first = -1;
-    auto find = [&](int j, const float *y) {
+    each([&](int j, const float *y) {
       int at = VEC;
 #pragma unroll
       for (int e = VEC - 1; e >= 0; --e)
         if (y[e] == m) at = e;
       const uint64_t hit = __ballot(at < VEC);
       if (first < 0 && hit) first = lane_value(first_index(j) + at, __builtin_ctzll(hit));
-    };
-    if constexpr (kHeld) {
-#pragma unroll
-      for (int j = 0; j < CHUNKS; ++j) find(j, x[j]);
-    } else {
-      for (int j = 0; j < chunks; ++j) {
-        float y[VEC];
-        load_logits<T>(row, first_index(j), V, y);
-        find(j, y);
-      }
-    }
+    });
     if constexpr (WAVES > 1) {
       g.sync();
       if (g.lane == 0) g.s.count[g.wave] = first;
@@ -680,7 +789,43 @@ __device__ __forceinline__ void sample_row(const RowGroup<WAVES> &g, const void 
     d = {first, 0.f};
   } else {
     Sampler<T, WAVES, CHUNKS> sampler(g, row, V, chunks, m, temperature, x);
-    d = sampler.draw(u, top_k, top_p, min_p);
+    if constexpr (FILTER && WAVES > 1) {
+      if (top_k > 0 && top_k < V && top_k <= kSampleFew) {
+        __shared__ __attribute__((aligned(16))) float s_few[kSampleFew];
+        __shared__ int s_index[kSampleFew];
+        __shared__ SampleShared<1> s_one;
+        const int n = sampler.gather_few(top_k, lowest, finite, s_few, s_index);
+        if (g.wave == 0) {
+          float few[kSampleFew / 256][4];
+          float least = kInf;
+#pragma unroll
+          for (int j = 0; j < kSampleFew / 256; ++j) {
+            const int i = (j * kWave + g.lane) * 4;
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(&s_few[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              few[j][e] = i + e < n ? y[e] : OT_NEG_INF;
+              least = fminf(least, i + e < n ? y[e] : kInf);
+            }
+          }
+          const RowGroup<1> one = {s_one, g.lane, 0};
+          float none = 0.f;
+          one.extremes(none, least);
+          Sampler<float, 1, kSampleFew / 256> rest(one, s_few, n, kSampleFew / 256, m, temperature, few);
+          rest.cut(top_k, top_p, min_p, least, n);
+          d = rest.draw(u);
+          if (g.lane == 0) {
+            *symbol = s_index[d.symbol];
+            *log_prob = d.log_prob;
+          }
+        }
+        g.sync();  // the few have been read
+        return;
+      }
+    }
+    if constexpr (FILTER) sampler.cut(top_k, top_p, min_p, lowest, finite);
+    else sampler.weigh();
+    d = sampler.draw(u);
   }
   g.sync();  // the group's shared values have been read
   if (g.thread() == 0) {
@@ -689,54 +834,95 @@ __device__ __forceinline__ void sample_row(const RowGroup<WAVES> &g, const void 
   }
 }
 
+// Waves per SIMD: as many as leave the elements of a thread in registers.
+constexpr int sample_occupancy(int waves, int elements) {
+  return waves == 16 || elements <= 8 ? 4 : waves == 4 && elements <= 16 ? 3 : waves == 1 ? 4 : 2;
+}
+
 // ROWS groups of WAVES waves per workgroup, a row each
-template <class T, int WAVES, int ROWS, int CHUNKS>
-__global__ __launch_bounds__(WAVES * ROWS * kWave, 4) void sample_kernel(
+template <class T, int WAVES, int ROWS, int CHUNKS, bool FILTER>
+__global__ __launch_bounds__(WAVES * ROWS * kWave, sample_occupancy(WAVES, CHUNKS * kSampleVec<T>)) void sample_kernel(
     const void *__restrict__ logits, int64_t row_stride, int64_t rows, int V, const float *__restrict__ uniform,
     SampleSettings set, int32_t *__restrict__ symbols, float *__restrict__ log_probs) {
   static_assert(ROWS == 1 || WAVES == 1, "barriers are per workgroup");
+  constexpr int VEC = kSampleVec<T>;
+  // short rows without cuts: the next row is on its way while one is worked on
+  constexpr bool kAhead = WAVES == 1 && !FILTER;
   __shared__ SampleShared<WAVES> s_row[ROWS];
   // the wave's number in scalar registers, and with it the row and its settings
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const RowGroup<WAVES> g = {s_row[ROWS > 1 ? wave : 0], (int)(threadIdx.x % kWave), ROWS > 1 ? 0 : wave};
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + (ROWS > 1 ? wave : 0); row < rows;
-       row += (int64_t)gridDim.x * ROWS) {
+  float x[CHUNKS > 0 ? CHUNKS : 1][VEC], next[kAhead ? CHUNKS : 1][VEC];
+  const int64_t stride = (int64_t)gridDim.x * ROWS;
+  auto load = [&](int64_t row, float (&to)[CHUNKS > 0 ? CHUNKS : 1][VEC]) {
+    if constexpr (CHUNKS > 0) {
+      const char *base = static_cast<const char *>(logits) + row * row_stride * (sizeof(T) == 4 ? 4 : 2);
+#pragma unroll
+      for (int j = 0; j < CHUNKS; ++j)
+        load_logits<T>(base, ((g.wave * CHUNKS + j) * kWave + g.lane) * VEC, V, to[j]);
+    }
+  };
+  int64_t row = (int64_t)blockIdx.x * ROWS + (ROWS > 1 ? wave : 0);
+  if constexpr (kAhead) {
+    if (row < rows) load(row, x);
+  }
+  for (; row < rows; row += stride) {
+    if constexpr (kAhead) load(min(row + stride, rows - 1), next);
+    else load(row, x);
     const char *base = static_cast<const char *>(logits) + row * row_stride * (sizeof(T) == 4 ? 4 : 2);
-    sample_row<T, WAVES, CHUNKS>(g, base, V, (double)uniform[row],
-                                 set.temperature ? set.temperature[row] : set.temperature_value,
-                                 set.top_k ? set.top_k[row] : set.top_k_value,
-                                 set.top_p ? set.top_p[row] : set.top_p_value,
-                                 set.min_p ? set.min_p[row] : set.min_p_value, symbols + row, log_probs + row);
+    sample_row<T, WAVES, CHUNKS, FILTER>(g, base, V, (double)uniform[row],
+                                         set.temperature ? set.temperature[row] : set.temperature_value,
+                                         set.top_k ? set.top_k[row] : set.top_k_value,
+                                         set.top_p ? set.top_p[row] : set.top_p_value,
+                                         set.min_p ? set.min_p[row] : set.min_p_value, x, symbols + row,
+                                         log_probs + row);
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int j = 0; j < CHUNKS; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[j][e] = next[j][e];
+    }
   }
 }
 
-template <class T, int WAVES, int ROWS, int CHUNKS>
+template <class T, int WAVES, int ROWS, int CHUNKS, bool FILTER>
 static int launch_sample_kernel(const void *logits, int64_t row_stride, int64_t rows, int32_t V,
                                 const float *uniform, const SampleSettings &set, int32_t *symbols,
                                 float *log_probs, hipStream_t s) {
   const int64_t groups = (rows + ROWS - 1) / ROWS;
-  const dim3 grid((unsigned)(groups < (1 << 20) ? groups : (1 << 20)));
-  hipLaunchKernelGGL((sample_kernel<T, WAVES, ROWS, CHUNKS>), grid, dim3(WAVES * ROWS * kWave), 0, s, logits,
-                     row_stride, rows, V, uniform, set, symbols, log_probs);
+  // with the next row on its way a wave takes many rows, as many waves as fit the chip
+  const int64_t most = WAVES == 1 && !FILTER ? kAheadGroups : 1 << 20;
+  const dim3 grid((unsigned)(groups < most ? groups : most));
+  hipLaunchKernelGGL((sample_kernel<T, WAVES, ROWS, CHUNKS, FILTER>), grid, dim3(WAVES * ROWS * kWave), 0, s,
+                     logits, row_stride, rows, V, uniform, set, symbols, log_probs);
   return (int)hipGetLastError();
 }
 
-template <class T>
+template <class T, bool FILTER>
 static int launch_sample(const void *logits, int64_t row_stride, int64_t rows, int32_t V, const float *uniform,
                          const SampleSettings &set, int32_t *symbols, float *log_probs, hipStream_t s) {
   constexpr int VEC = kSampleVec<T>, kChunk = kWave * VEC;  // 256 or 512 elements
-#define OT_SAMPLE(WAVES_, ROWS_, CHUNKS_)                                                              \
-  return launch_sample_kernel<T, WAVES_, ROWS_, CHUNKS_>(logits, row_stride, rows, V, uniform, set, symbols, \
-                                                         log_probs, s)
+#define OT_SAMPLE(WAVES_, ROWS_, CHUNKS_)                                                                       \
+  return launch_sample_kernel<T, WAVES_, ROWS_, CHUNKS_, FILTER>(logits, row_stride, rows, V, uniform, set, symbols, \
+                                                                 log_probs, s)
   if (V <= kChunk) OT_SAMPLE(1, 4, 1);
   if (V <= 2 * kChunk) OT_SAMPLE(1, 4, 2);
   if (V <= 2048) OT_SAMPLE(4, 1, 2048 / 4 / kChunk);
   if (V <= 4096) OT_SAMPLE(4, 1, 4096 / 4 / kChunk);
   if (V <= 6144) OT_SAMPLE(4, 1, 6144 / 4 / kChunk);
+  if (V <= 8192) OT_SAMPLE(8, 1, 8192 / 8 / kChunk);
   if (V <= 16384) OT_SAMPLE(16, 1, 16384 / 16 / kChunk);
-  if (V <= 32768) OT_SAMPLE(16, 1, 32768 / 16 / kChunk);
   OT_SAMPLE(16, 1, 0);
 #undef OT_SAMPLE
+}
+
+template <class T>
+static int launch_sample(const void *logits, int64_t row_stride, int64_t rows, int32_t V, const float *uniform,
+                         const SampleSettings &set, int32_t *symbols, float *log_probs, hipStream_t s) {
+  const bool filter = set.top_k || set.top_p || set.min_p || (set.top_k_value > 0 && set.top_k_value < V) ||
+                      set.top_p_value < 1.f || set.min_p_value > 0.f;
+  return filter ? launch_sample<T, true>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, s)
+                : launch_sample<T, false>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, s);
 }
 
 }  // namespace ot
