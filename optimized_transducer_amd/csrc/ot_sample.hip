@@ -43,7 +43,6 @@ struct SampleSettings {
 
 constexpr int kSampleBins = 256;
 constexpr int kSampleFew = 512;  // entries that one wave takes over from the others
-constexpr int64_t kAheadGroups = 256 * 7;  // workgroups of 4 rows
 constexpr float kInf = __builtin_huge_valf();
 
 // ---- wave-wide helpers ----------------------------------------------------------------------
@@ -186,6 +185,13 @@ __device__ __forceinline__ void load_logits(const void *row, int i, int V, float
   }
 }
 
+// ln(2)^k / k! for k = 11 down to 1: read once into scalar registers, where literals would be moved
+// into vector registers in front of every use
+__constant__ double kExpSeries[11] = {4.4455382718708115e-10, 7.0549116208011233e-09, 1.0178086009239699e-07,
+                                      1.3215486790144307e-06, 1.5252733804059841e-05, 1.5403530393381609e-04,
+                                      1.3333558146428443e-03, 9.6181291076284772e-03, 5.5504108664821580e-02,
+                                      2.4022650695910072e-01, 6.9314718055994531e-01};
+
 // exp((x - m) / T) = 2^n * 2^f with n the nearest integer to (x - m) * c, c = log2(e) / T, and
 // 2^f the exponential series of f * ln 2, |f| <= 1/2, up to the 11th power (the next term is
 // below 2^-47).  Exactly 1 at x = m, exactly 0 at x = -inf.
@@ -195,18 +201,9 @@ struct Weight {
   __device__ __forceinline__ double operator()(float x) const {
     // (T = inf and x = -inf make a NaN of the product, which fmax drops)
     const double t = __builtin_fmax(((double)x - m) * c, -1100.0), n = __builtin_rint(t), f = t - n;
-    // ln(2)^k / k!
-    double p = 4.4455382718708115e-10;
-    p = __builtin_fma(p, f, 7.0549116208011233e-09);
-    p = __builtin_fma(p, f, 1.0178086009239699e-07);
-    p = __builtin_fma(p, f, 1.3215486790144307e-06);
-    p = __builtin_fma(p, f, 1.5252733804059841e-05);
-    p = __builtin_fma(p, f, 1.5403530393381609e-04);
-    p = __builtin_fma(p, f, 1.3333558146428443e-03);
-    p = __builtin_fma(p, f, 9.6181291076284772e-03);
-    p = __builtin_fma(p, f, 5.5504108664821580e-02);
-    p = __builtin_fma(p, f, 2.4022650695910072e-01);
-    p = __builtin_fma(p, f, 6.9314718055994531e-01);
+    double p = kExpSeries[0];
+#pragma unroll
+    for (int k = 1; k < 11; ++k) p = __builtin_fma(p, f, kExpSeries[k]);
     p = __builtin_fma(p, f, 1.0);
     return __builtin_ldexp(p, (int)n);
   }
@@ -223,6 +220,14 @@ struct Drawn {
   int symbol;
   float log_prob;
 };
+
+// (x - m) / T - log(total); the largest entry always remains, so total = 1 + the others' sum
+__device__ __forceinline__ float log_probability(float logit, float m, float T, double total) {
+  const float rest = (float)(total - 1.0), t = 1.0f + rest;
+  const float small = logf(t) + (rest - (t - 1.0f)) / t;
+  const float z = m - logit > 3e38f || T < 1e-30f || T > 1e30f ? (float)(((double)logit - m) / T) : (logit - m) / T;
+  return z - (rest < 1.0f ? small : logf((float)total));
+}
 
 // Draws from a row with a finite largest entry m at a temperature above 0.  Every thread of the
 // group calls it with the same arguments and gets the same answer.
@@ -601,6 +606,57 @@ struct Sampler {
     }
   }
 
+  // Where the running sum, `run` in front of chunk j, passes the target in it: in the first lane
+  // whose sum does, else the last one with a weight, and there in the first element that does,
+  // else the last one with a weight (sums in another order can fall short of each other's borders
+  // by their rounding).  mine, upto: the lane's sum and the scan over the lanes.
+  __device__ __forceinline__ void find(const double t[VEC], const float *y, int i, double run, double mine, double upto,
+                                       double target, uint64_t pass, uint64_t some, int &symbol, float &logit) const {
+    const int l = pass ? __builtin_ctzll(pass) : 63 - __builtin_clzll(some);
+    double c = run + (upto - mine);
+    int at = -1;
+    bool found = false;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const double next = c + t[e];
+      if (!found && t[e] > 0.0) {
+        at = e;
+        found = next > target;
+      }
+      c = next;
+    }
+    // (a maximum, and not a choice between elements, which would index the registers)
+    float at_logit = OT_NEG_INF;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) at_logit = fmaxf(at_logit, e == at ? y[e] : OT_NEG_INF);
+    symbol = lane_value(i + at, l);
+    logit = lane_value(at_logit, l);
+  }
+
+  // the same as draw() for one wave that holds the row's weights: one scan per chunk
+  __device__ __forceinline__ void draw_alone(double u, int &symbol, float &logit, double &total) const {
+    double mine[CHUNKS], upto[CHUNKS], before[CHUNKS + 1];
+    before[0] = 0.0;
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) {
+      mine[j] = pairwise(w[j]);
+      upto[j] = wave_scan(mine[j]);
+      before[j + 1] = before[j] + lane_value(upto[j], kWave - 1);
+    }
+    total = before[CHUNKS];
+    // u >= 1, or a product that rounds up to the total, takes the last entry with a weight
+    const double target = fmax(u, 0.0) * total;
+    const bool past = !(target < total);
+    symbol = -1;
+#pragma unroll
+    for (int j = CHUNKS - 1; j >= 0; --j) {
+      const uint64_t some = __ballot(mine[j] > 0.0);
+      if (past ? symbol < 0 && some != 0 : before[j] <= target && target < before[j + 1])
+        find(w[j], x[j], first_index(j), before[j], mine[j], upto[j], target,
+             __ballot(before[j] + upto[j] > target), some, symbol, logit);
+    }
+  }
+
   __device__ __forceinline__ Drawn draw(double u) {
     // totals of the waves' parts, then the part, the chunk, the lane and the element in which
     // the running sum passes u * total
@@ -643,28 +699,7 @@ struct Sampler {
         const uint64_t pass = __ballot(run + upto > target);
         const uint64_t some = __ballot(mine > 0.0);
         if (some) {
-          // the first lane whose running sum passes the target, else the last with a weight;
-          // in that lane the first element that does, else its last with a weight (sums in
-          // another order can fall short of each other's borders by their rounding)
-          const int l = pass ? __builtin_ctzll(pass) : 63 - __builtin_clzll(some);
-          double c = run + (upto - mine);
-          int at = -1;
-          bool found = false;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const double next = c + t[e];
-            if (!found && t[e] > 0.0) {
-              at = e;
-              found = next > target;
-            }
-            c = next;
-          }
-          // (a maximum, and not a choice between elements, which would index the registers)
-          float at_logit = OT_NEG_INF;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) at_logit = fmaxf(at_logit, e == at ? y[e] : OT_NEG_INF);
-          last = lane_value(i + at, l);
-          last_logit = lane_value(at_logit, l);
+          find(t, y, i, run, mine, upto, target, pass, some, last, last_logit);
           if (pass) symbol = last;
         }
         run += chunk;
@@ -700,21 +735,37 @@ struct Sampler {
       }
       logit = load_element<T>(row, symbol);
     }
-    return {symbol, log_prob(logit, total)};
+    return {symbol, log_probability(logit, m, T_, total)};
   }
 
-  // (x - m) / T - log(total); the largest entry always remains, so total = 1 + the others' sum
-  __device__ __forceinline__ float log_prob(float logit, double total) const {
-    const float rest = (float)(total - 1.0), t = 1.0f + rest;
-    const float small = logf(t) + (rest - (t - 1.0f)) / t;
-    const float z = m - logit > 3e38f || T_ < 1e-30f || T_ > 1e30f ? (float)(((double)logit - m) / T_) : (logit - m) / T_;
-    return z - (rest < 1.0f ? small : logf((float)total));
-  }
 };
 
+// What the cuts start from: the largest entry m, whether there is a NaN (bad < 0), the smallest
+// finite entry and how many are finite; of elements, and of the group.
+template <int VEC>
+__device__ __forceinline__ void look(const float *y, float &m, float &bad, float &lowest, int &finite) {
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    m = fmaxf(m, y[e]);
+    if (y[e] != y[e]) bad = -1.f;
+    if (y[e] > OT_NEG_INF) {
+      lowest = fminf(lowest, y[e]);
+      ++finite;
+    }
+  }
+}
+template <int WAVES>
+__device__ __forceinline__ void look_together(const RowGroup<WAVES> &g, float &m, float &bad, float &lowest,
+                                              int &finite) {
+  float none = 0.f;
+  double nothing = 0.0;
+  g.extremes(none, bad);
+  g.extremes(m, lowest);
+  g.totals(nothing, finite);
+}
+
 // One row, in x if it is held: settles the rows without an answer and the greedy ones, draws from
-// the others.  FILTER: one of top_k, top_p and min_p may be in force.  Where top_k leaves few
-// entries of a row of several waves, one wave goes on with them alone.
+// the others.  FILTER: one of top_k, top_p and min_p may be in force.
 template <class T, int WAVES, int CHUNKS, bool FILTER>
 __device__ __forceinline__ void sample_row(const RowGroup<WAVES> &g, const void *row, int V, double u,
                                            float temperature, int top_k, float top_p, float min_p,
@@ -740,22 +791,8 @@ __device__ __forceinline__ void sample_row(const RowGroup<WAVES> &g, const void 
   float m = OT_NEG_INF, bad = 0.f, lowest = kInf;
   int finite = 0;
   if (cuts) {
-    each([&](int, const float *y) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        m = fmaxf(m, y[e]);
-        if (y[e] != y[e]) bad = -1.f;
-        if (y[e] > OT_NEG_INF) {
-          lowest = fminf(lowest, y[e]);
-          ++finite;
-        }
-      }
-    });
-    float none = 0.f;
-    double nothing = 0.0;
-    g.extremes(none, bad);
-    g.extremes(m, lowest);
-    g.totals(nothing, finite);
+    each([&](int, const float *y) { look<VEC>(y, m, bad, lowest, finite); });
+    look_together(g, m, bad, lowest, finite);
   } else {
     each([&](int, const float *y) {
 #pragma unroll
@@ -789,40 +826,6 @@ __device__ __forceinline__ void sample_row(const RowGroup<WAVES> &g, const void 
     d = {first, 0.f};
   } else {
     Sampler<T, WAVES, CHUNKS> sampler(g, row, V, chunks, m, temperature, x);
-    if constexpr (FILTER && WAVES > 1) {
-      if (top_k > 0 && top_k < V && top_k <= kSampleFew) {
-        __shared__ __attribute__((aligned(16))) float s_few[kSampleFew];
-        __shared__ int s_index[kSampleFew];
-        __shared__ SampleShared<1> s_one;
-        const int n = sampler.gather_few(top_k, lowest, finite, s_few, s_index);
-        if (g.wave == 0) {
-          float few[kSampleFew / 256][4];
-          float least = kInf;
-#pragma unroll
-          for (int j = 0; j < kSampleFew / 256; ++j) {
-            const int i = (j * kWave + g.lane) * 4;
-            const f32x4 y = *reinterpret_cast<const f32x4 *>(&s_few[i]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              few[j][e] = i + e < n ? y[e] : OT_NEG_INF;
-              least = fminf(least, i + e < n ? y[e] : kInf);
-            }
-          }
-          const RowGroup<1> one = {s_one, g.lane, 0};
-          float none = 0.f;
-          one.extremes(none, least);
-          Sampler<float, 1, kSampleFew / 256> rest(one, s_few, n, kSampleFew / 256, m, temperature, few);
-          rest.cut(top_k, top_p, min_p, least, n);
-          d = rest.draw(u);
-          if (g.lane == 0) {
-            *symbol = s_index[d.symbol];
-            *log_prob = d.log_prob;
-          }
-        }
-        g.sync();  // the few have been read
-        return;
-      }
-    }
     if constexpr (FILTER) sampler.cut(top_k, top_p, min_p, lowest, finite);
     else sampler.weigh();
     d = sampler.draw(u);
@@ -834,9 +837,208 @@ __device__ __forceinline__ void sample_row(const RowGroup<WAVES> &g, const void 
   }
 }
 
+// Rows of several waves of which top_k leaves few entries (0 < top_k <= kSampleFew, top_k < V):
+// the waves of a workgroup find them together, for BATCH rows one after the other, and then a wave
+// each goes on with the few of one row.
+template <class T, int WAVES, int CHUNKS, int BATCH>
+__global__ __launch_bounds__(WAVES * kWave, WAVES == 16 ? 4 : WAVES == 8 || CHUNKS * kSampleVec<T> > 16 ? 2 : 3) void
+sample_few_kernel(const void *__restrict__ logits, int64_t row_stride, int64_t rows, int V,
+                  const float *__restrict__ uniform, SampleSettings set, int32_t *__restrict__ symbols,
+                  float *__restrict__ log_probs) {
+  static_assert(BATCH <= WAVES, "a wave takes one row");
+  constexpr int VEC = kSampleVec<T>, kLanes = kSampleFew / 256;
+  __shared__ SampleShared<WAVES> s_all;
+  __shared__ SampleShared<1> s_one[BATCH];
+  __shared__ __attribute__((aligned(16))) float s_few[BATCH][kSampleFew];
+  __shared__ int s_index[BATCH][kSampleFew];
+  __shared__ float s_m[BATCH];
+  __shared__ int s_n[BATCH];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const RowGroup<WAVES> g = {s_all, lane, wave};
+  const int chunks = CHUNKS > 0 ? CHUNKS : (V + WAVES * kWave * VEC - 1) / (WAVES * kWave * VEC);
+  const int top_k = set.top_k_value;
+  for (int64_t row0 = (int64_t)blockIdx.x * BATCH; row0 < rows; row0 += (int64_t)gridDim.x * BATCH) {
+#pragma unroll 1
+    for (int q = 0; q < BATCH && row0 + q < rows; ++q) {
+      const char *base =
+          static_cast<const char *>(logits) + (row0 + q) * row_stride * (sizeof(T) == 4 ? 4 : 2);
+      float x[CHUNKS > 0 ? CHUNKS : 1][VEC];
+      float m = OT_NEG_INF, bad = 0.f, lowest = kInf;
+      int finite = 0;
+      if constexpr (CHUNKS > 0) {
+#pragma unroll
+        for (int j = 0; j < CHUNKS; ++j) load_logits<T>(base, ((wave * CHUNKS + j) * kWave + lane) * VEC, V, x[j]);
+#pragma unroll
+        for (int j = 0; j < CHUNKS; ++j) look<VEC>(x[j], m, bad, lowest, finite);
+      } else {
+        for (int j = 0; j < chunks; ++j) {
+          float y[VEC];
+          load_logits<T>(base, ((wave * chunks + j) * kWave + lane) * VEC, V, y);
+          look<VEC>(y, m, bad, lowest, finite);
+        }
+      }
+      look_together(g, m, bad, lowest, finite);
+      int n = -1;
+      if (!(bad < 0.f || __builtin_isinf(m))) {
+        Sampler<T, WAVES, CHUNKS> sampler(g, base, V, chunks, m, 1.0f, x);
+        n = sampler.gather_few(top_k, lowest, finite, s_few[q], s_index[q]);
+      }
+      if (g.thread() == 0) {
+        s_m[q] = m;
+        s_n[q] = n;
+      }
+    }
+    g.sync();
+    if (wave < BATCH && row0 + wave < rows) {
+      const int64_t row = row0 + wave;
+      const double u = uniform[row];
+      const float temperature = set.temperature ? set.temperature[row] : set.temperature_value;
+      const float top_p = set.top_p ? set.top_p[row] : set.top_p_value;
+      const float min_p = set.min_p ? set.min_p[row] : set.min_p_value;
+      const int n = s_n[wave];
+      const float m = s_m[wave];
+      Drawn d = {-1, OT_NEG_INF};
+      if (n > 0 && u == u) {
+        float few[kLanes][4], lowest = kInf;
+#pragma unroll
+        for (int j = 0; j < kLanes; ++j) {
+          const int i = (j * kWave + lane) * 4;
+          const f32x4 y = *reinterpret_cast<const f32x4 *>(&s_few[wave][i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            few[j][e] = i + e < n ? y[e] : OT_NEG_INF;
+            lowest = fminf(lowest, i + e < n ? y[e] : kInf);
+          }
+        }
+        const RowGroup<1> one = {s_one[wave], lane, 0};
+        if (!(temperature > 0.f)) {
+#pragma unroll
+          for (int j = kLanes - 1; j >= 0; --j) {
+            int at = 4;
+#pragma unroll
+            for (int e = 3; e >= 0; --e)
+              if (few[j][e] == m) at = e;
+            const uint64_t hit = __ballot(at < 4);
+            if (hit) d = {lane_value((j * kWave + lane) * 4 + at, __builtin_ctzll(hit)), 0.f};
+          }
+        } else {
+          float none = 0.f;
+          one.extremes(none, lowest);
+          Sampler<float, 1, kLanes> rest(one, s_few[wave], n, kLanes, m, temperature, few);
+          rest.cut(top_k, top_p, min_p, lowest, n);
+          d = rest.draw(u);
+        }
+        d.symbol = s_index[wave][d.symbol];
+      }
+      if (lane == 0) {
+        symbols[row] = d.symbol;
+        log_probs[row] = d.log_prob;
+      }
+    }
+    g.sync();  // the few have been read
+  }
+}
+
+template <class T, int WAVES, int CHUNKS, int BATCH>
+static int launch_sample_few(const void *logits, int64_t row_stride, int64_t rows, int32_t V, const float *uniform,
+                             const SampleSettings &set, int32_t *symbols, float *log_probs, hipStream_t s) {
+  const int64_t groups = (rows + BATCH - 1) / BATCH;
+  const dim3 grid((unsigned)(groups < (1 << 20) ? groups : (1 << 20)));
+  hipLaunchKernelGGL((sample_few_kernel<T, WAVES, CHUNKS, BATCH>), grid, dim3(WAVES * kWave), 0, s, logits, row_stride,
+                     rows, V, uniform, set, symbols, log_probs);
+  return (int)hipGetLastError();
+}
+
+// Short rows without cuts: a wave per row, `batch` rows (64 at most) one after the other with the
+// next one on its way, their numbers and settings read and their answers written side by side, and
+// the logarithms of a batch taken at once, a row per lane.
+template <class T, int CHUNKS>
+__global__ __launch_bounds__(kBlock, 4) void sample_plain_kernel(const void *__restrict__ logits, int64_t row_stride,
+                                                                 int64_t rows, int V, int batch,
+                                                                 const float *__restrict__ uniform,
+                                                                 const float *__restrict__ temperature,
+                                                                 float temperature_value,
+                                                                 int32_t *__restrict__ symbols,
+                                                                 float *__restrict__ log_probs) {
+  constexpr int VEC = kSampleVec<T>;
+  __shared__ SampleShared<1> s_unused[1];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const RowGroup<1> g = {s_unused[0], (int)(threadIdx.x % kWave), 0};
+  auto load = [&](int64_t row, float (&to)[CHUNKS][VEC]) {
+    const char *base = static_cast<const char *>(logits) + min(row, rows - 1) * row_stride * (sizeof(T) == 4 ? 4 : 2);
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) load_logits<T>(base, (j * kWave + g.lane) * VEC, V, to[j]);
+  };
+  const int64_t stride = (int64_t)gridDim.x * kWavesPerBlock * batch;
+  int64_t row0 = ((int64_t)blockIdx.x * kWavesPerBlock + wave) * batch;
+  if (row0 >= rows) return;
+  float x[CHUNKS][VEC];
+  load(row0, x);
+  for (; row0 < rows; row0 += stride) {
+    const int n = (int)min((int64_t)batch, rows - row0);
+    const float my_u = g.lane < n ? uniform[row0 + g.lane] : 0.f;
+    const float my_T = temperature && g.lane < n ? temperature[row0 + g.lane] : temperature_value;
+    int my_symbol = -1;
+    float my_logit = 0.f, my_m = 0.f;
+    double my_total = 1.0;
+#pragma unroll 1
+    for (int q = 0; q < n; ++q) {
+      float next[CHUNKS][VEC];
+      load(q + 1 < n ? row0 + q + 1 : row0 + stride, next);
+      float m = OT_NEG_INF;
+      bool nan = false;
+#pragma unroll
+      for (int j = 0; j < CHUNKS; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          m = fmaxf(m, x[j][e]);
+          nan |= x[j][e] != x[j][e];
+        }
+      m = group_allreduce<kWave>(m, MaxOp());
+      const float u = lane_value(my_u, q), T_ = lane_value(my_T, q);
+      int symbol = -1;
+      float logit = m;
+      double total = 1.0;
+      if (__ballot(nan) || __builtin_isinf(m) || u != u) {
+        // no answer
+      } else if (!(T_ > 0.f)) {
+#pragma unroll
+        for (int j = CHUNKS - 1; j >= 0; --j) {
+          int at = VEC;
+#pragma unroll
+          for (int e = VEC - 1; e >= 0; --e)
+            if (x[j][e] == m) at = e;
+          const uint64_t hit = __ballot(at < VEC);
+          if (hit) symbol = lane_value((j * kWave + g.lane) * VEC + at, __builtin_ctzll(hit));
+        }
+      } else {
+        Sampler<T, 1, CHUNKS> sampler(g, nullptr, V, CHUNKS, m, T_, x);
+        sampler.weigh();
+        sampler.draw_alone((double)u, symbol, logit, total);
+      }
+      if (g.lane == q) {
+        my_symbol = symbol;
+        my_logit = logit;
+        my_m = m;
+        my_total = total;
+      }
+#pragma unroll
+      for (int j = 0; j < CHUNKS; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[j][e] = next[j][e];
+    }
+    if (g.lane < n) {
+      symbols[row0 + g.lane] = my_symbol;
+      log_probs[row0 + g.lane] = my_symbol < 0 ? OT_NEG_INF
+                                 : my_T > 0.f  ? log_probability(my_logit, my_m, my_T, my_total)
+                                               : 0.f;
+    }
+  }
+}
+
 // Waves per SIMD: as many as leave the elements of a thread in registers.
 constexpr int sample_occupancy(int waves, int elements) {
-  return waves == 16 || elements <= 8 ? 4 : waves == 4 && elements <= 16 ? 3 : waves == 1 ? 4 : 2;
+  return waves == 16 || waves == 1 ? 4 : waves == 4 && elements <= 16 ? 3 : 2;
 }
 
 // ROWS groups of WAVES waves per workgroup, a row each
@@ -846,42 +1048,25 @@ __global__ __launch_bounds__(WAVES * ROWS * kWave, sample_occupancy(WAVES, CHUNK
     SampleSettings set, int32_t *__restrict__ symbols, float *__restrict__ log_probs) {
   static_assert(ROWS == 1 || WAVES == 1, "barriers are per workgroup");
   constexpr int VEC = kSampleVec<T>;
-  // short rows without cuts: the next row is on its way while one is worked on
-  constexpr bool kAhead = WAVES == 1 && !FILTER;
   __shared__ SampleShared<WAVES> s_row[ROWS];
   // the wave's number in scalar registers, and with it the row and its settings
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const RowGroup<WAVES> g = {s_row[ROWS > 1 ? wave : 0], (int)(threadIdx.x % kWave), ROWS > 1 ? 0 : wave};
-  float x[CHUNKS > 0 ? CHUNKS : 1][VEC], next[kAhead ? CHUNKS : 1][VEC];
+  float x[CHUNKS > 0 ? CHUNKS : 1][VEC];
   const int64_t stride = (int64_t)gridDim.x * ROWS;
-  auto load = [&](int64_t row, float (&to)[CHUNKS > 0 ? CHUNKS : 1][VEC]) {
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + (ROWS > 1 ? wave : 0); row < rows; row += stride) {
+    const char *base = static_cast<const char *>(logits) + row * row_stride * (sizeof(T) == 4 ? 4 : 2);
     if constexpr (CHUNKS > 0) {
-      const char *base = static_cast<const char *>(logits) + row * row_stride * (sizeof(T) == 4 ? 4 : 2);
 #pragma unroll
       for (int j = 0; j < CHUNKS; ++j)
-        load_logits<T>(base, ((g.wave * CHUNKS + j) * kWave + g.lane) * VEC, V, to[j]);
+        load_logits<T>(base, ((g.wave * CHUNKS + j) * kWave + g.lane) * VEC, V, x[j]);
     }
-  };
-  int64_t row = (int64_t)blockIdx.x * ROWS + (ROWS > 1 ? wave : 0);
-  if constexpr (kAhead) {
-    if (row < rows) load(row, x);
-  }
-  for (; row < rows; row += stride) {
-    if constexpr (kAhead) load(min(row + stride, rows - 1), next);
-    else load(row, x);
-    const char *base = static_cast<const char *>(logits) + row * row_stride * (sizeof(T) == 4 ? 4 : 2);
     sample_row<T, WAVES, CHUNKS, FILTER>(g, base, V, (double)uniform[row],
                                          set.temperature ? set.temperature[row] : set.temperature_value,
                                          set.top_k ? set.top_k[row] : set.top_k_value,
                                          set.top_p ? set.top_p[row] : set.top_p_value,
                                          set.min_p ? set.min_p[row] : set.min_p_value, x, symbols + row,
                                          log_probs + row);
-    if constexpr (kAhead) {
-#pragma unroll
-      for (int j = 0; j < CHUNKS; ++j)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) x[j][e] = next[j][e];
-    }
   }
 }
 
@@ -890,11 +1075,22 @@ static int launch_sample_kernel(const void *logits, int64_t row_stride, int64_t 
                                 const float *uniform, const SampleSettings &set, int32_t *symbols,
                                 float *log_probs, hipStream_t s) {
   const int64_t groups = (rows + ROWS - 1) / ROWS;
-  // with the next row on its way a wave takes many rows, as many waves as fit the chip
-  const int64_t most = WAVES == 1 && !FILTER ? kAheadGroups : 1 << 20;
-  const dim3 grid((unsigned)(groups < most ? groups : most));
+  const dim3 grid((unsigned)(groups < (1 << 20) ? groups : (1 << 20)));
   hipLaunchKernelGGL((sample_kernel<T, WAVES, ROWS, CHUNKS, FILTER>), grid, dim3(WAVES * ROWS * kWave), 0, s,
                      logits, row_stride, rows, V, uniform, set, symbols, log_probs);
+  return (int)hipGetLastError();
+}
+
+template <class T, int CHUNKS>
+static int launch_sample_plain(const void *logits, int64_t row_stride, int64_t rows, int32_t V, const float *uniform,
+                               const SampleSettings &set, int32_t *symbols, float *log_probs, hipStream_t s) {
+  // 7 waves per SIMD of 256 compute units are resident; 16 rows a batch fill a line of answers
+  constexpr int64_t kWaves = 256 * 4 * 7;
+  const int batch = (int)(rows <= kWaves ? 1 : rows >= 16 * kWaves ? 16 : (rows + kWaves - 1) / kWaves);
+  const int64_t per_group = (int64_t)kWavesPerBlock * batch, groups = (rows + per_group - 1) / per_group;
+  const dim3 grid((unsigned)(groups < kWaves / kWavesPerBlock ? groups : kWaves / kWavesPerBlock));
+  hipLaunchKernelGGL((sample_plain_kernel<T, CHUNKS>), grid, dim3(kBlock), 0, s, logits, row_stride, rows, V, batch,
+                     uniform, set.temperature, set.temperature_value, symbols, log_probs);
   return (int)hipGetLastError();
 }
 
@@ -905,8 +1101,34 @@ static int launch_sample(const void *logits, int64_t row_stride, int64_t rows, i
 #define OT_SAMPLE(WAVES_, ROWS_, CHUNKS_)                                                                       \
   return launch_sample_kernel<T, WAVES_, ROWS_, CHUNKS_, FILTER>(logits, row_stride, rows, V, uniform, set, symbols, \
                                                                  log_probs, s)
-  if (V <= kChunk) OT_SAMPLE(1, 4, 1);
-  if (V <= 2 * kChunk) OT_SAMPLE(1, 4, 2);
+#define OT_SAMPLE_FEW(WAVES_, CHUNKS_, BATCH_)                                                              \
+  return launch_sample_few<T, WAVES_, CHUNKS_, BATCH_>(logits, row_stride, rows, V, uniform, set, symbols, \
+                                                       log_probs, s)
+  if constexpr (FILTER) {
+    if (V > 2 * kChunk && !set.top_k && set.top_k_value > 0 && set.top_k_value <= kSampleFew) {
+      // a batch of rows per workgroup where there are rows for all compute units
+      if (rows >= 2048) {
+        if (V <= 2048) OT_SAMPLE_FEW(4, 2048 / 4 / kChunk, 4);
+        if (V <= 4096) OT_SAMPLE_FEW(4, 4096 / 4 / kChunk, 4);
+        if (V <= 6144) OT_SAMPLE_FEW(4, 6144 / 4 / kChunk, 4);
+      }
+      if (V <= 2048) OT_SAMPLE_FEW(4, 2048 / 4 / kChunk, 1);
+      if (V <= 4096) OT_SAMPLE_FEW(4, 4096 / 4 / kChunk, 1);
+      if (V <= 8192) OT_SAMPLE_FEW(8, 8192 / 8 / kChunk, 1);
+      if (V <= 16384) OT_SAMPLE_FEW(16, 16384 / 16 / kChunk, 1);
+      OT_SAMPLE_FEW(16, 0, 1);
+    }
+  }
+#undef OT_SAMPLE_FEW
+  if constexpr (FILTER) {
+    if (V <= kChunk) OT_SAMPLE(1, 4, 1);
+    if (V <= 2 * kChunk) OT_SAMPLE(1, 4, 2);
+  } else {
+    if (V <= kChunk)
+      return launch_sample_plain<T, 1>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, s);
+    if (V <= 2 * kChunk)
+      return launch_sample_plain<T, 2>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, s);
+  }
   if (V <= 2048) OT_SAMPLE(4, 1, 2048 / 4 / kChunk);
   if (V <= 4096) OT_SAMPLE(4, 1, 4096 / 4 / kChunk);
   if (V <= 6144) OT_SAMPLE(4, 1, 6144 / 4 / kChunk);
