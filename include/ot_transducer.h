@@ -517,14 +517,24 @@ int ot_joiner_project_blocks(const void *x, const float *x_scale,
  *
  * logits (rows, V) of `dtype` (any of the three), element (r, v) at
  * logits[r * row_stride + v]; uniform, symbols, log_probs (rows).  Each setting
- * is one value, or (pointer not NULL) one per row.  rows = 0 does nothing. */
+ * is one value, or (pointer not NULL) one per row.  rows = 0 does nothing.
+ *
+ * A caller may lend ot_sample_symbols_workspace_bytes(rows, V, with_top_k)
+ * bytes, 16-byte aligned, contents irrelevant before and after (with_top_k:
+ * whether top_k is given or top_k_value is within (0, V)): long rows (V above
+ * 16384, up to 524288) without top_k are then done in slices, a workgroup
+ * each.  With a NULL or short workspace a workgroup does a row: the same
+ * answers, except where two sums of 64 bits in another order part. */
+size_t ot_sample_symbols_workspace_bytes(int64_t rows, int32_t V,
+                                         int32_t with_top_k);
 int ot_sample_symbols(const void *logits, int32_t dtype, int64_t row_stride,
                       int64_t rows, int32_t V, const float *uniform,
                       const float *temperature, float temperature_value,
                       const int32_t *top_k, int32_t top_k_value,
                       const float *top_p, float top_p_value,
                       const float *min_p, float min_p_value, int32_t *symbols,
-                      float *log_probs, void *stream);
+                      float *log_probs, void *workspace,
+                      size_t workspace_bytes, void *stream);
 
 /* Plain device-to-device copy kernel of n floats; used to calibrate profiler
  * byte counters against a transfer of known size. */

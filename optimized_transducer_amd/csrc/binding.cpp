@@ -977,6 +977,10 @@ std::pair<torch::Tensor, torch::Tensor> sample_symbols(
   const torch::Tensor q = row_setting(min_p, torch::kFloat, logits, "min_p");
   torch::Tensor symbols = torch::empty({rows}, logits.options().dtype(torch::kInt32));
   torch::Tensor log_probs = torch::empty({rows}, logits.options().dtype(torch::kFloat));
+  const size_t ws_bytes = ot_sample_symbols_workspace_bytes(
+      rows, (int32_t)V, k.defined() || (top_k_value > 0 && top_k_value < V));
+  torch::Tensor workspace;
+  if (ws_bytes > 0) workspace = torch::empty({(int64_t)ws_bytes}, logits.options().dtype(torch::kUInt8));
   ScopedTimer timer("sample_symbols", stream);
   OT_CHECK(ot_sample_symbols(
       logits.data_ptr(), dtype, logits.stride(0), rows, (int32_t)V, uniform.data_ptr<float>(),
@@ -984,7 +988,7 @@ std::pair<torch::Tensor, torch::Tensor> sample_symbols(
       k.defined() ? k.data_ptr<int32_t>() : nullptr, (int32_t)std::min<int64_t>(top_k_value, INT32_MAX),
       p.defined() ? p.data_ptr<float>() : nullptr, (float)top_p_value,
       q.defined() ? q.data_ptr<float>() : nullptr, (float)min_p_value, symbols.data_ptr<int32_t>(),
-      log_probs.data_ptr<float>(), stream));
+      log_probs.data_ptr<float>(), ws_bytes > 0 ? workspace.data_ptr() : nullptr, ws_bytes, stream));
   return {symbols, log_probs};
 }
 

@@ -657,7 +657,9 @@ struct Sampler {
     }
   }
 
-  __device__ __forceinline__ Drawn draw(double u) {
+  // `start`, `whole`: what lies in front of these entries and the total, where they are a slice of
+  // a row
+  __device__ __forceinline__ Drawn draw(double u, double start = 0.0, double whole = -1.0) {
     // totals of the waves' parts, then the part, the chunk, the lane and the element in which
     // the running sum passes u * total
     if (!part_known) {
@@ -670,19 +672,21 @@ struct Sampler {
       });
       part = wave_sum(part);
     }
-    double total = part, before = 0.0;
+    double total = start + part, before = start;
     if constexpr (WAVES > 1) {
       g.sync();
       if (g.lane == 0) g.s.sum[g.wave] = part;
       if (g.thread() == 0) g.s.index = -1;
       g.sync();
-      total = 0.0;
+      total = start;
       for (int k = 0; k < WAVES; ++k) {
         if (k == g.wave) before = total;
         total += g.s.sum[k];
       }
     }
-    const double target = fmax(u, 0.0) * total;
+    if (whole >= 0.0) total = whole;
+    const double product = fmax(u, 0.0) * total;
+    const double target = product < total ? product : __builtin_huge_val();
     int symbol = -1;
     float logit = 0.f;
     if (before <= target && target < before + part) {  // one wave
@@ -1036,6 +1040,457 @@ __global__ __launch_bounds__(kBlock, 4) void sample_plain_kernel(const void *__r
   }
 }
 
+// ---- long rows in slices ---------------------------------------------------------------------
+//
+// A row beyond the registers of a workgroup is cut into slices of kSlice entries, a workgroup
+// each, so that few rows fill the chip too and every step reads the row once:
+//   1 facts   a slice's largest entry, where it is, and the sum of its weights relative to it
+//   2 bins    (top_p) weights of a slice by value, in 1024 bins of equal width, as integers of
+//             2^-32: sums that no order of the additions changes
+//   3 join    (top_p) a workgroup per row: the bin in which the weights of all slices reach top_p
+//             of the total
+//   4 cuts    (top_p, min_p) of a slice, the 64-bit sums of what lies above that bin, and the
+//             entries in it, in index order
+//   5 draw    a workgroup per row: the exact cut among the entries of the bin, the slice in which
+//             the running sum passes u times what remains, and the symbol in that slice
+// Where a bin holds more than kBinEntries of a slice, or the rounded sums missed the bin, step 5
+// does the row in the way of the shorter ones, reading it in every step.
+
+constexpr float kBinScale = 4294967040.f;  // the largest below 2^32
+constexpr int kSlice = 8192, kSliceBins = 1024, kBinEntries = 256;
+constexpr int kSliceWaves = 8, kSliceThreads = kSliceWaves * kWave;
+constexpr int kMostSlices = kWave;     // of a row: a lane each
+constexpr int64_t kSliceRows = 256;  // rows whose slices are in the workspace at a time
+
+struct SliceFacts {
+  double sum;
+  float m, bad;
+  int first, unused;
+};
+struct SliceCut {
+  double above, kept;  // sums of the weights above the bin: all of them, and those that min_p leaves
+  int entries, unused;
+};
+struct BinEntry {
+  float x;
+  int index;
+};
+
+// A batch of rows and the workspace of their slices.
+struct SlicedRows {
+  const void *logits;
+  int64_t row_stride, row0;  // first row of the batch
+  int V, slices;
+  const float *uniform;
+  SampleSettings set;
+  SliceFacts *facts;   // (rows, slices)
+  unsigned long long *bins;  // (rows, slices, kSliceBins)
+  SliceCut *cuts;      // (rows, slices)
+  BinEntry *entries;   // (rows, slices, kBinEntries)
+  int *cut_bin;        // (rows)
+  bool binned, cut;    // steps 2 and 3, and step 4, are run
+};
+
+// What the slices of a row come to, the same in every wave; lane k holds slice k.
+struct RowState {
+  float m, T, from, per_unit;
+  float slice_m;
+  int slice_first;
+  double slice_sum;  // of its weights, relative to m
+  bool answer, greedy, cuts;
+  double want;
+
+  __device__ __forceinline__ RowState(const SlicedRows &a, int64_t r, int lane) {
+    const int64_t row = a.row0 + r;
+    SliceFacts f = {0.0, OT_NEG_INF, 0.f, -1, 0};
+    if (lane < a.slices) f = a.facts[r * a.slices + lane];
+    slice_m = f.m;
+    slice_first = f.first;
+    T = a.set.temperature ? a.set.temperature[row] : a.set.temperature_value;
+    const float top_p = a.set.top_p ? a.set.top_p[row] : a.set.top_p_value, u = a.uniform[row];
+    greedy = !(T > 0.f);
+    m = group_allreduce<kWave>(f.m, MaxOp());
+    const bool bad = __ballot(f.bad < 0.f) != 0;
+    answer = !(bad || __builtin_isinf(m) || u != u);
+    cuts = answer && !greedy && top_p < 1.f;
+    slice_sum = want = 0.0;
+    from = OT_NEG_INF;
+    per_unit = 0.f;
+    if (!answer || greedy) return;
+    const Weight weight(m, T);
+    slice_sum = f.sum * weight(f.m);
+    if (!cuts) return;
+    const double p = fmaxf(top_p, 0.f), total = wave_sum(slice_sum);
+    want = p * total;
+    // entries of weights below (1 - p) * total / V come to less than what lies behind the cut
+    const float z = __log2f((float)fmax((1.0 - p) * total / a.V * 0.99, 1e-30)) / (float)weight.c;
+    from = z > -1e30f ? fminf(m, m + 1.001f * z) : -3.4e38f;
+    const float half = 0.5f * m - 0.5f * from;
+    if (half > 1e-30f) per_unit = (0.5f * kSliceBins) / half;
+  }
+  // 0 for the largest entries; kSliceBins below `from`
+  __device__ __forceinline__ int bin(float y) const {
+    return y < from ? kSliceBins : (int)fminf((m - y) * per_unit, kSliceBins - 1.0f);
+  }
+};
+
+template <class T>
+struct Slice {
+  static constexpr int VEC = kSampleVec<T>, CHUNKS = kSlice / kSliceThreads / VEC;
+  typedef Sampler<T, kSliceWaves, CHUNKS> S;
+  float x[CHUNKS][VEC];
+  const void *base;
+  int V;  // entries
+
+  // thread t's elements: as Sampler holds them
+  __device__ __forceinline__ Slice(const SlicedRows &a, int64_t r, int slice, int lane, int wave) {
+    const int64_t first = (a.row0 + r) * a.row_stride + (int64_t)slice * kSlice;
+    base = static_cast<const char *>(a.logits) + first * (sizeof(T) == 4 ? 4 : 2);
+    V = min(kSlice, a.V - slice * kSlice);
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) load_logits<T>(base, index(j, lane, wave), V, x[j]);
+  }
+  __device__ __forceinline__ static int index(int j, int lane, int wave) {
+    return ((wave * CHUNKS + j) * kWave + lane) * VEC;
+  }
+};
+
+#define OT_SLICE_GROUP                                                                         \
+  __shared__ SampleShared<kSliceWaves> s_all;                                               \
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave; \
+  const RowGroup<kSliceWaves> g = {s_all, lane, wave}
+
+template <class T>
+__global__ __launch_bounds__(kSliceThreads, 4) void slice_facts_kernel(SlicedRows a) {
+  typedef Slice<T> P;
+  OT_SLICE_GROUP;
+  const int slice = blockIdx.x;
+  const int64_t r = blockIdx.y;
+  const P p(a, r, slice, lane, wave);
+  float m = OT_NEG_INF, bad = 0.f;
+#pragma unroll
+  for (int j = 0; j < P::CHUNKS; ++j)
+#pragma unroll
+    for (int e = 0; e < P::VEC; ++e) {
+      m = fmaxf(m, p.x[j][e]);
+      if (p.x[j][e] != p.x[j][e]) bad = -1.f;
+    }
+  g.extremes(m, bad);
+  const float T_ = a.set.temperature ? a.set.temperature[a.row0 + r] : a.set.temperature_value;
+  double sum = 0.0;
+  int first = 0x7fffffff, none = 0;
+  if (!__builtin_isinf(m)) {
+#pragma unroll
+    for (int j = P::CHUNKS - 1; j >= 0; --j)
+#pragma unroll
+      for (int e = P::VEC - 1; e >= 0; --e)
+        if (p.x[j][e] == m) first = P::index(j, lane, wave) + e;
+    if (T_ > 0.f) {
+      const Weight weight(m, T_);
+#pragma unroll
+      for (int j = 0; j < P::CHUNKS; ++j) {
+        double t[P::VEC];
+#pragma unroll
+        for (int e = 0; e < P::VEC; ++e) t[e] = weight(p.x[j][e]);
+        sum += P::S::pairwise(t);
+      }
+    }
+  }
+  g.totals(sum, none);
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) first = min(first, __shfl_xor(first, d, kWave));
+  g.sync();
+  if (lane == 0) s_all.count[wave] = first;
+  g.sync();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < kSliceWaves; ++k) first = min(first, s_all.count[k]);
+    a.facts[r * a.slices + slice] = {sum, m, bad, first == 0x7fffffff ? -1 : slice * kSlice + first, 0};
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(kSliceThreads, 4) void slice_bins_kernel(SlicedRows a) {
+  typedef Slice<T> P;
+  __shared__ unsigned long long s_bins[kSliceBins];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int64_t r = blockIdx.y;
+  const RowState st(a, r, lane);
+  if (!st.cuts) return;
+  for (int i = threadIdx.x; i < kSliceBins; i += kSliceThreads) s_bins[i] = 0;
+  const P p(a, r, blockIdx.x, lane, wave);
+  const float per_octave = (float)Weight(st.m, st.T).c;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < P::CHUNKS; ++j)
+#pragma unroll
+    for (int e = 0; e < P::VEC; ++e)
+      if (p.x[j][e] >= st.from) {
+        // (a NaN, of a temperature that 32 bits do not hold, is 0)
+        const float v = fmaxf(__builtin_amdgcn_exp2f((p.x[j][e] - st.m) * per_octave) * kBinScale, 0.f);
+        atomicAdd(&s_bins[st.bin(p.x[j][e])], (unsigned long long)(unsigned)v);
+      }
+  __syncthreads();
+  unsigned long long *to = a.bins + (r * a.slices + blockIdx.x) * kSliceBins;
+  for (int i = threadIdx.x; i < kSliceBins; i += kSliceThreads) to[i] = s_bins[i];
+}
+
+// thread t looks at bin t
+__global__ __launch_bounds__(kSliceBins) void slice_join_kernel(SlicedRows a) {
+  constexpr int kWaves = kSliceBins / kWave;
+  __shared__ unsigned long long s_sum[kWaves];
+  __shared__ int s_bin;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t r = blockIdx.x;
+  const RowState st(a, r, lane);
+  if (!st.cuts) return;
+  const unsigned long long *from = a.bins + r * a.slices * kSliceBins + threadIdx.x;
+  unsigned long long amount = 0;
+  for (int k = 0; k < a.slices; ++k) amount += from[k * kSliceBins];
+  unsigned long long upto = amount;
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const unsigned long long v = __shfl_up(upto, d, kWave);
+    if (lane >= d) upto += v;
+  }
+  if (lane == kWave - 1) s_sum[wave] = upto;
+  if (threadIdx.x == 0) s_bin = kSliceBins - 1;
+  __syncthreads();
+  for (int k = 0; k < wave; ++k) upto += s_sum[k];
+  if (amount > 0 && (double)upto >= st.want * (double)kBinScale) atomicMin(&s_bin, (int)threadIdx.x);
+  __syncthreads();
+  if (threadIdx.x == 0) a.cut_bin[r] = s_bin;
+}
+
+template <class T>
+__global__ __launch_bounds__(kSliceThreads, 4) void slice_cuts_kernel(SlicedRows a) {
+  typedef Slice<T> P;
+  OT_SLICE_GROUP;
+  const int slice = blockIdx.x;
+  const int64_t r = blockIdx.y;
+  const RowState st(a, r, lane);
+  if (!st.answer || st.greedy) return;
+  const int cut_bin = st.cuts ? a.cut_bin[r] : kSliceBins;  // (all entries are above that)
+  const P p(a, r, slice, lane, wave);
+  const float min_p_row = a.set.min_p ? a.set.min_p[a.row0 + r] : a.set.min_p_value;
+  const double least = min_p_row > 0.f ? fminf(min_p_row, 1.f) : 0.0;
+  const Weight weight(st.m, st.T);
+  double above = 0.0, kept = 0.0;
+  int here = 0, none = 0;
+#pragma unroll
+  for (int j = 0; j < P::CHUNKS; ++j) {
+    double t[P::VEC], l[P::VEC];
+#pragma unroll
+    for (int e = 0; e < P::VEC; ++e) {
+      const float y = p.x[j][e];
+      const int b = !(y > OT_NEG_INF) ? kSliceBins + 1 : st.cuts ? st.bin(y) : 0;
+      t[e] = b < cut_bin ? weight(y) : 0.0;
+      l[e] = t[e] >= least ? t[e] : 0.0;
+      here += __popcll(__ballot(b == cut_bin));
+    }
+    above += P::S::pairwise(t);
+    kept += P::S::pairwise(l);
+  }
+  g.totals(above, none);
+  g.totals(kept, none);
+  // entries of the bin, in index order
+  __syncthreads();
+  if (lane == 0) s_all.count[wave] = here;
+  __syncthreads();
+  int at = 0, total = 0;
+  for (int k = 0; k < kSliceWaves; ++k) {
+    if (k == wave) at = total;
+    total += s_all.count[k];
+  }
+  if (st.cuts && total > 0 && total <= kBinEntries) {
+    BinEntry *to = a.entries + (r * a.slices + slice) * kBinEntries;
+#pragma unroll
+    for (int j = 0; j < P::CHUNKS; ++j) {
+      int place = at;
+      bool in[P::VEC];
+#pragma unroll
+      for (int e = 0; e < P::VEC; ++e) {  // entries of the lanes before
+        in[e] = st.bin(p.x[j][e]) == cut_bin;
+        const uint64_t which = __ballot(in[e]);
+        place += __builtin_amdgcn_mbcnt_hi((unsigned)(which >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)which, 0));
+        at += __popcll(which);
+      }
+#pragma unroll
+      for (int e = 0; e < P::VEC; ++e)
+        if (in[e]) to[place++] = {p.x[j][e], slice * kSlice + P::index(j, lane, wave) + e};
+    }
+  }
+  if (threadIdx.x == 0) a.cuts[r * a.slices + slice] = {above, kept, total, 0};
+}
+
+template <class T>
+__global__ __launch_bounds__(kSliceThreads, 2) void slice_draw_kernel(SlicedRows a, int32_t *__restrict__ symbols,
+                                                               float *__restrict__ log_probs) {
+  typedef Slice<T> P;
+  OT_SLICE_GROUP;
+  constexpr int kMost = 2048;  // entries of the bin of all slices
+  __shared__ BinEntry s_entry[kMost];
+  __shared__ double s_weight[kMost];
+  __shared__ float s_cut;
+  __shared__ unsigned s_best;
+  __shared__ int s_last;
+  const int64_t r = blockIdx.x, row = a.row0 + r;
+  const RowState st(a, r, lane);
+  if (!st.answer || st.greedy) {
+    const uint64_t at = __ballot(st.slice_m == st.m);
+    const int first = at ? lane_value(st.slice_first, __builtin_ctzll(at)) : -1;
+    if (threadIdx.x == 0) {
+      symbols[row] = st.answer ? first : -1;
+      log_probs[row] = st.answer ? 0.f : OT_NEG_INF;
+    }
+    return;
+  }
+  const double u = a.uniform[row];
+  const float min_p_row = a.set.min_p ? a.set.min_p[row] : a.set.min_p_value;
+  const float top_p = a.set.top_p ? a.set.top_p[row] : a.set.top_p_value;
+  const double least = min_p_row > 0.f ? fminf(min_p_row, 1.f) : 0.0;
+  const Weight weight(st.m, st.T);
+  SliceCut mine = {0.0, st.slice_sum, 0, 0};  // of this lane's slice
+  if (a.cut) mine = lane < a.slices ? a.cuts[r * a.slices + lane] : SliceCut{0.0, 0.0, 0, 0};
+  float cut = OT_NEG_INF;  // entries above it remain, and those at it up to index `last`
+  int last = 0x7fffffff;
+  if (st.cuts) {
+    const int upto = wave_scan(mine.entries), from = upto - mine.entries, n = lane_value(upto, kWave - 1);
+    const double above = wave_sum(mine.above);
+    bool slow = n > kMost || __ballot(mine.entries > kBinEntries) != 0;
+    if (!slow) {
+      if (threadIdx.x == 0) {
+        s_best = 0;
+        s_last = -1;
+      }
+      for (int k = 0; k < a.slices; ++k) {
+        const int to = lane_value(from, k), c = lane_value(mine.entries, k);
+        for (int i = threadIdx.x; i < c; i += kSliceThreads) {
+          const BinEntry e = a.entries[(r * a.slices + k) * kBinEntries + i];
+          s_entry[to + i] = e;
+          s_weight[to + i] = weight(e.x);
+        }
+      }
+      __syncthreads();
+      // of the values of the bin, the largest that the cut can be at
+      auto about = [&](int i, double &sum, int &same, int &earlier) {
+        const float x = s_entry[i].x;
+        sum = 0.0;
+        same = earlier = 0;
+        for (int k = 0; k < n; ++k) {
+          const float y = s_entry[k].x;
+          sum += y > x ? s_weight[k] : 0.0;
+          same += y == x;
+          earlier += y == x && k < i;
+        }
+        sum += above;
+      };
+      for (int i = threadIdx.x; i < n; i += kSliceThreads) {
+        double sum;
+        int same, earlier;
+        about(i, sum, same, earlier);
+        const double with = sum + same * s_weight[i];
+        if ((sum < st.want || s_entry[i].x == st.m) && with >= st.want) atomicMax(&s_best, order_key(s_entry[i].x));
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < n; i += kSliceThreads) {
+        const float x = s_entry[i].x;
+        if (order_key(x) != s_best) continue;
+        double sum;
+        int same, earlier;
+        about(i, sum, same, earlier);
+        // number `earlier` of those at the cut remains if sum + earlier * weight < want
+        const double w = s_weight[i], q = w > 0.0 ? ceil((st.want - sum) / w) : same;
+        const int keep = max(q < same ? (int)q : same, x == st.m ? 1 : 0);
+        if (earlier == 0) s_cut = x;
+        if (earlier < keep) atomicMax(&s_last, s_entry[i].index);
+      }
+      __syncthreads();
+      slow = s_best == 0;
+    }
+    if (slow) {
+      float unused[1][P::VEC];
+      const char *base = static_cast<const char *>(a.logits) + row * a.row_stride * (sizeof(T) == 4 ? 4 : 2);
+      sample_row<T, kSliceWaves, 0, true>(g, base, a.V, u, st.T, 0, top_p, min_p_row, unused, symbols + row,
+                                             log_probs + row);
+      return;
+    }
+    cut = s_cut;
+    last = s_last;
+    // what remains of the bin in this lane's slice
+    for (int i = from; i < upto; ++i) {
+      const BinEntry e = s_entry[i];
+      if ((e.x > cut || (e.x == cut && e.index <= last)) && s_weight[i] >= least) mine.kept += s_weight[i];
+    }
+  }
+  // the slice in which the running sum passes the target; u >= 1: the last one with a weight
+  const double run = wave_scan(mine.kept), total = lane_value(run, kWave - 1);
+  const uint64_t some = __ballot(mine.kept > 0.0), pass = __ballot(mine.kept > 0.0 && run > fmax(u, 0.0) * total);
+  const int slice = pass ? __builtin_ctzll(pass) : 63 - __builtin_clzll(some);
+  const double before = slice > 0 ? lane_value(run, slice - 1) : 0.0;
+  P p(a, r, slice, lane, wave);
+  if (st.cuts) {
+#pragma unroll
+    for (int j = 0; j < P::CHUNKS; ++j)
+#pragma unroll
+      for (int e = 0; e < P::VEC; ++e)
+        if (p.x[j][e] < cut || (p.x[j][e] == cut && slice * kSlice + P::index(j, lane, wave) + e > last))
+          p.x[j][e] = OT_NEG_INF;
+  }
+  typename P::S sampler(g, p.base, p.V, P::CHUNKS, st.m, st.T, p.x);
+  sampler.weigh();
+  if (least > 0.0) sampler.keep_min_p((float)least);
+  const Drawn d = sampler.draw(u, before, total);
+  if (threadIdx.x == 0) {
+    symbols[row] = slice * kSlice + d.symbol;
+    log_probs[row] = d.log_prob;
+  }
+}
+#undef OT_SLICE_GROUP
+
+// Bytes of workspace for a row (the arrays' elements need 8-byte alignment).
+static size_t slice_row_bytes(int32_t V) {
+  const size_t slices = ((size_t)V + kSlice - 1) / kSlice;
+  return sizeof(int64_t) + slices * (sizeof(SliceFacts) + sizeof(SliceCut) + kSliceBins * sizeof(unsigned long long) + kBinEntries * sizeof(BinEntry));
+}
+
+template <class T>
+static int launch_slices(const void *logits, int64_t row_stride, int64_t rows, int32_t V, const float *uniform,
+                         const SampleSettings &set, int32_t *symbols, float *log_probs, void *workspace,
+                         hipStream_t s) {
+  SlicedRows a;
+  a.logits = logits;
+  a.row_stride = row_stride;
+  a.V = V;
+  a.slices = (V + kSlice - 1) / kSlice;
+  a.uniform = uniform;
+  a.set = set;
+  const int64_t most = rows < kSliceRows ? rows : kSliceRows;
+  char *at = static_cast<char *>(workspace);
+  a.facts = reinterpret_cast<SliceFacts *>(at);
+  at += (size_t)most * a.slices * sizeof(SliceFacts);
+  a.cuts = reinterpret_cast<SliceCut *>(at);
+  at += (size_t)most * a.slices * sizeof(SliceCut);
+  a.entries = reinterpret_cast<BinEntry *>(at);
+  at += (size_t)most * a.slices * kBinEntries * sizeof(BinEntry);
+  a.bins = reinterpret_cast<unsigned long long *>(at);
+  at += (size_t)most * a.slices * kSliceBins * sizeof(unsigned long long);
+  a.cut_bin = reinterpret_cast<int *>(at);
+  a.binned = set.top_p || set.top_p_value < 1.f;
+  a.cut = a.binned || set.min_p || set.min_p_value > 0.f;
+  for (a.row0 = 0; a.row0 < rows; a.row0 += kSliceRows) {
+    const unsigned n = (unsigned)(rows - a.row0 < kSliceRows ? rows - a.row0 : kSliceRows);
+    const dim3 grid((unsigned)a.slices, n), block(kSliceThreads);
+    hipLaunchKernelGGL((slice_facts_kernel<T>), grid, block, 0, s, a);
+    if (a.binned) {
+      hipLaunchKernelGGL((slice_bins_kernel<T>), grid, block, 0, s, a);
+      hipLaunchKernelGGL(slice_join_kernel, dim3(n), dim3(kSliceBins), 0, s, a);
+    }
+    if (a.cut) hipLaunchKernelGGL((slice_cuts_kernel<T>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((slice_draw_kernel<T>), dim3(n), block, 0, s, a, symbols, log_probs);
+  }
+  return (int)hipGetLastError();
+}
+
 // Waves per SIMD: as many as leave the elements of a thread in registers.
 constexpr int sample_occupancy(int waves, int elements) {
   return waves == 16 || waves == 1 ? 4 : waves == 4 && elements <= 16 ? 3 : 2;
@@ -1140,7 +1595,9 @@ static int launch_sample(const void *logits, int64_t row_stride, int64_t rows, i
 
 template <class T>
 static int launch_sample(const void *logits, int64_t row_stride, int64_t rows, int32_t V, const float *uniform,
-                         const SampleSettings &set, int32_t *symbols, float *log_probs, hipStream_t s) {
+                         const SampleSettings &set, int32_t *symbols, float *log_probs, void *workspace,
+                         hipStream_t s) {
+  if (workspace) return launch_slices<T>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, workspace, s);
   const bool filter = set.top_k || set.top_p || set.min_p || (set.top_k_value > 0 && set.top_k_value < V) ||
                       set.top_p_value < 1.f || set.min_p_value > 0.f;
   return filter ? launch_sample<T, true>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, s)
@@ -1151,11 +1608,18 @@ static int launch_sample(const void *logits, int64_t row_stride, int64_t rows, i
 
 using namespace ot;
 
-extern "C" int ot_sample_symbols(const void *logits, int32_t dtype, int64_t row_stride, int64_t rows, int32_t V,
-                                 const float *uniform, const float *temperature, float temperature_value,
-                                 const int32_t *top_k, int32_t top_k_value, const float *top_p,
-                                 float top_p_value, const float *min_p, float min_p_value, int32_t *symbols,
-                                 float *log_probs, void *stream) {
+extern "C" {
+
+size_t ot_sample_symbols_workspace_bytes(int64_t rows, int32_t V, int32_t with_top_k) {
+  if (rows <= 0 || V <= 16384 || V > kMostSlices * kSlice || with_top_k) return 0;
+  return (size_t)(rows < kSliceRows ? rows : kSliceRows) * slice_row_bytes(V);
+}
+
+int ot_sample_symbols(const void *logits, int32_t dtype, int64_t row_stride, int64_t rows, int32_t V,
+                      const float *uniform, const float *temperature, float temperature_value, const int32_t *top_k,
+                      int32_t top_k_value, const float *top_p, float top_p_value, const float *min_p,
+                      float min_p_value, int32_t *symbols, float *log_probs, void *workspace, size_t workspace_bytes,
+                      void *stream) {
   if (rows == 0) return 0;
   if (!logits || !uniform || !symbols || !log_probs || rows < 0 || rows > INT32_MAX || V <= 0 ||
       V > INT32_MAX - 4096 || row_stride < 0)
@@ -1169,8 +1633,17 @@ extern "C" int ot_sample_symbols(const void *logits, int32_t dtype, int64_t row_
   const SampleSettings set = {temperature, top_p,       min_p,       top_k,
                               temperature_value, top_p_value, min_p_value, top_k_value};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == OT_DTYPE_F32) return launch_sample<float>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, s);
-  if (dtype == OT_DTYPE_F16) return launch_sample<F16>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, s);
-  if (dtype == OT_DTYPE_BF16) return launch_sample<BF16>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, s);
+  const size_t need =
+      ot_sample_symbols_workspace_bytes(rows, V, top_k || (top_k_value > 0 && top_k_value < V));
+  void *ws = need > 0 && workspace_bytes >= need ? workspace : nullptr;
+  if (reinterpret_cast<uintptr_t>(ws) & 15) return OT_E_MISALIGNED;
+  if (dtype == OT_DTYPE_F32)
+    return launch_sample<float>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, ws, s);
+  if (dtype == OT_DTYPE_F16)
+    return launch_sample<F16>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, ws, s);
+  if (dtype == OT_DTYPE_BF16)
+    return launch_sample<BF16>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, ws, s);
   return OT_E_BAD_ARG;
 }
+
+}  // extern "C"

@@ -119,9 +119,14 @@ def test_c_abi_refuses_bad_arguments():
     def sample(logits=one, dtype=0, stride=10, rows=4, V=10, uniform=one, t=null, k=null, p=null, m=null,
                symbols=one, log_probs=one):
         return L.ot_sample_symbols(logits, i32(dtype), i64(stride), i64(rows), i32(V), uniform, t, f32(1), k,
-                                   i32(0), p, f32(1), m, f32(0), symbols, log_probs, null)
+                                   i32(0), p, f32(1), m, f32(0), symbols, log_probs, null, size(0), null)
 
     assert sample(rows=0) == 0
+    L.ot_sample_symbols_workspace_bytes.restype = size
+    need = L.ot_sample_symbols_workspace_bytes
+    assert need(i64(4), i32(500), i32(0)) == 0 and need(i64(0), i32(50000), i32(0)) == 0
+    assert need(i64(4), i32(50000), i32(1)) == 0 and need(i64(4), i32(50000), i32(0)) > 0
+    assert need(i64(1 << 20), i32(50000), i32(0)) == need(i64(256), i32(50000), i32(0))
     for bad in (dict(logits=null), dict(uniform=null), dict(symbols=null), dict(log_probs=null), dict(rows=-1),
                 dict(rows=1 << 31), dict(V=0), dict(V=2 ** 31 - 1), dict(stride=-1), dict(dtype=5)):
         assert sample(**bad) == -1, bad
