@@ -1245,6 +1245,7 @@ __global__ __launch_bounds__(kSliceBins) void slice_join_kernel(SlicedRows a) {
   if (!st.cuts) return;
   const unsigned long long *from = a.bins + r * a.slices * kSliceBins + threadIdx.x;
   unsigned long long amount = 0;
+#pragma unroll 8
   for (int k = 0; k < a.slices; ++k) amount += from[k * kSliceBins];
   unsigned long long upto = amount;
 #pragma unroll
@@ -1362,47 +1363,49 @@ __global__ __launch_bounds__(kSliceThreads, 2) void slice_draw_kernel(SlicedRows
         s_best = 0;
         s_last = -1;
       }
-      for (int k = 0; k < a.slices; ++k) {
+      for (int k = wave; k < a.slices; k += kSliceWaves) {
         const int to = lane_value(from, k), c = lane_value(mine.entries, k);
-        for (int i = threadIdx.x; i < c; i += kSliceThreads) {
+        for (int i = lane; i < c; i += kWave) {
           const BinEntry e = a.entries[(r * a.slices + k) * kBinEntries + i];
           s_entry[to + i] = e;
           s_weight[to + i] = weight(e.x);
         }
       }
       __syncthreads();
-      // of the values of the bin, the largest that the cut can be at
-      auto about = [&](int i, double &sum, int &same, int &earlier) {
+      // of each entry: the weights above it, the entries equal to it, and those of them before it
+      constexpr int kPer = kMost / kSliceThreads;
+      double sum[kPer];
+      int same[kPer], earlier[kPer];
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        const int i = q * kSliceThreads + threadIdx.x;
+        sum[q] = above;
+        same[q] = earlier[q] = 0;
+        if (i >= n) continue;
         const float x = s_entry[i].x;
-        sum = 0.0;
-        same = earlier = 0;
+#pragma unroll 8
         for (int k = 0; k < n; ++k) {
           const float y = s_entry[k].x;
-          sum += y > x ? s_weight[k] : 0.0;
-          same += y == x;
-          earlier += y == x && k < i;
+          const double w = s_weight[k];
+          sum[q] += y > x ? w : 0.0;
+          same[q] += y == x;
+          earlier[q] += y == x && k < i;
         }
-        sum += above;
-      };
-      for (int i = threadIdx.x; i < n; i += kSliceThreads) {
-        double sum;
-        int same, earlier;
-        about(i, sum, same, earlier);
-        const double with = sum + same * s_weight[i];
-        if ((sum < st.want || s_entry[i].x == st.m) && with >= st.want) atomicMax(&s_best, order_key(s_entry[i].x));
+        // the cut: the largest value that it can be at (roundings could make it two)
+        if ((sum[q] < st.want || x == st.m) && sum[q] + same[q] * s_weight[i] >= st.want)
+          atomicMax(&s_best, order_key(x));
       }
       __syncthreads();
-      for (int i = threadIdx.x; i < n; i += kSliceThreads) {
-        const float x = s_entry[i].x;
-        if (order_key(x) != s_best) continue;
-        double sum;
-        int same, earlier;
-        about(i, sum, same, earlier);
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        const int i = q * kSliceThreads + threadIdx.x;
+        if (i >= n || order_key(s_entry[i].x) != s_best) continue;
         // number `earlier` of those at the cut remains if sum + earlier * weight < want
-        const double w = s_weight[i], q = w > 0.0 ? ceil((st.want - sum) / w) : same;
-        const int keep = max(q < same ? (int)q : same, x == st.m ? 1 : 0);
-        if (earlier == 0) s_cut = x;
-        if (earlier < keep) atomicMax(&s_last, s_entry[i].index);
+        const float x = s_entry[i].x;
+        const double w = s_weight[i], j = w > 0.0 ? ceil((st.want - sum[q]) / w) : same[q];
+        const int keep = max(j < same[q] ? (int)j : same[q], x == st.m ? 1 : 0);
+        if (earlier[q] == 0) s_cut = x;
+        if (earlier[q] < keep) atomicMax(&s_last, s_entry[i].index);
       }
       __syncthreads();
       slow = s_best == 0;
