@@ -21,10 +21,20 @@
 // No sort: a cut is found by a histogram of the interval that still holds it, 256 bins at a
 // time, until one value is left; two levels do for rows without many equal values.
 //
-// A row is worked on by one wave (short rows: its elements stay in registers, four rows per
-// workgroup and no barrier), by 4 or 16 waves with the elements in registers, or by 16 waves
-// that read it again in each step (long rows, served by the caches).  Every wave owns a
-// contiguous part of the row, so that a running sum needs one number from each wave.
+// Who works on a row (what bounds it; times at T = 1 and sigma 2):
+//   a wave                short rows, up to 512 (float32) or 1024 elements, in registers, and no
+//                         barrier.  Without cuts a wave takes a batch of them: the 64-bit weights
+//                         bound it (751 992 x 500 float32 0.49 ms, 3.1 TB/s)
+//   4, 8 or 16 waves      rows up to 16384, in registers; of all the waves only the wide steps
+//                         profit, so that the barriers and scans of the cuts bound it.  A top_k of
+//                         512 at most is found by all of them, and one wave goes on with what is left
+//                         (20 011 x 5000 float16 with all cuts 0.46 ms, 0.72 with all waves to the end)
+//   slices                longer rows, several workgroups each (64 x 131 072 bfloat16, top_p: 69 us,
+//                         266 by a workgroup per row; launches and the chain of steps bound it)
+//   16 waves              rows beyond the slices, or with top_k: they read the row in every step,
+//                         served by the caches
+// Every wave owns a contiguous part of the row, so that a running sum needs one number from each
+// wave.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -1059,8 +1069,9 @@ __global__ __launch_bounds__(kBlock, 4) void sample_plain_kernel(const void *__r
 constexpr float kBinScale = 4294967040.f;  // the largest below 2^32
 constexpr int kSlice = 8192, kSliceBins = 1024, kBinEntries = 256;
 constexpr int kSliceWaves = 8, kSliceThreads = kSliceWaves * kWave;
-constexpr int kMostSlices = kWave;     // of a row: a lane each
-constexpr int64_t kSliceRows = 256;  // rows whose slices are in the workspace at a time
+constexpr int kMostSlices = kWave;    // of a row: a lane each
+constexpr int kLongRow = 16384;       // the longest row that a workgroup holds in registers
+constexpr int64_t kSliceRows = 256;   // rows whose slices are in the workspace at a time
 
 struct SliceFacts {
   double sum;
@@ -1083,12 +1094,12 @@ struct SlicedRows {
   int V, slices;
   const float *uniform;
   SampleSettings set;
-  SliceFacts *facts;   // (rows, slices)
+  SliceFacts *facts;         // (rows, slices)
   unsigned long long *bins;  // (rows, slices, kSliceBins)
-  SliceCut *cuts;      // (rows, slices)
-  BinEntry *entries;   // (rows, slices, kBinEntries)
-  int *cut_bin;        // (rows)
-  bool binned, cut;    // steps 2 and 3, and step 4, are run
+  int *cut_bin;              // (rows)
+  SliceCut *cuts;            // (rows, slices)
+  BinEntry *entries;         // (rows, slices, kBinEntries)
+  bool binned, cut;          // steps 2 and 3, and step 4, are run
 };
 
 // What the slices of a row come to, the same in every wave; lane k holds slice k.
@@ -1155,8 +1166,8 @@ struct Slice {
   }
 };
 
-#define OT_SLICE_GROUP                                                                         \
-  __shared__ SampleShared<kSliceWaves> s_all;                                               \
+#define OT_SLICE_GROUP                                                                              \
+  __shared__ SampleShared<kSliceWaves> s_all;                                                       \
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave; \
   const RowGroup<kSliceWaves> g = {s_all, lane, wave}
 
@@ -1325,7 +1336,7 @@ __global__ __launch_bounds__(kSliceThreads, 4) void slice_cuts_kernel(SlicedRows
 
 template <class T>
 __global__ __launch_bounds__(kSliceThreads, 2) void slice_draw_kernel(SlicedRows a, int32_t *__restrict__ symbols,
-                                                               float *__restrict__ log_probs) {
+                                                                      float *__restrict__ log_probs) {
   typedef Slice<T> P;
   OT_SLICE_GROUP;
   constexpr int kMost = 2048;  // entries of the bin of all slices
@@ -1414,7 +1425,7 @@ __global__ __launch_bounds__(kSliceThreads, 2) void slice_draw_kernel(SlicedRows
       float unused[1][P::VEC];
       const char *base = static_cast<const char *>(a.logits) + row * a.row_stride * (sizeof(T) == 4 ? 4 : 2);
       sample_row<T, kSliceWaves, 0, true>(g, base, a.V, u, st.T, 0, top_p, min_p_row, unused, symbols + row,
-                                             log_probs + row);
+                                          log_probs + row);
       return;
     }
     cut = s_cut;
@@ -1453,7 +1464,8 @@ __global__ __launch_bounds__(kSliceThreads, 2) void slice_draw_kernel(SlicedRows
 // Bytes of workspace for a row (the arrays' elements need 8-byte alignment).
 static size_t slice_row_bytes(int32_t V) {
   const size_t slices = ((size_t)V + kSlice - 1) / kSlice;
-  return sizeof(int64_t) + slices * (sizeof(SliceFacts) + sizeof(SliceCut) + kSliceBins * sizeof(unsigned long long) + kBinEntries * sizeof(BinEntry));
+  return sizeof(int64_t) + slices * (sizeof(SliceFacts) + sizeof(SliceCut) +
+                                     kSliceBins * sizeof(unsigned long long) + kBinEntries * sizeof(BinEntry));
 }
 
 template <class T>
@@ -1600,9 +1612,17 @@ template <class T>
 static int launch_sample(const void *logits, int64_t row_stride, int64_t rows, int32_t V, const float *uniform,
                          const SampleSettings &set, int32_t *symbols, float *log_probs, void *workspace,
                          hipStream_t s) {
-  if (workspace) return launch_slices<T>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, workspace, s);
-  const bool filter = set.top_k || set.top_p || set.min_p || (set.top_k_value > 0 && set.top_k_value < V) ||
-                      set.top_p_value < 1.f || set.min_p_value > 0.f;
+  const bool with_top_p = set.top_p || set.top_p_value < 1.f, with_min_p = set.min_p || set.min_p_value > 0.f;
+  // Slices or one workgroup of 16 waves (us, float32, slices first):
+  //   top_p     64 x 20 000 37 / 62, 4096 x 20 000 820 / 939, 64 x 131 072 69 / 337,
+  //             1024 x 131 072 656 / 1485; 64 x 16 000 (elements in registers) 35 / 40, 4096 732 / 646
+  //   no cuts   64 x 20 000 12 / 13, 4096 x 20 000 275 / 198, 64 x 50 000 14 / 26, 4096 x 50 000 425 / 469,
+  //             64 x 131 072 19 / 54
+  //   min_p     64 x 20 000 18 / 16, 64 x 50 000 23 / 31, 256 x 50 000 51 / 38, 64 x 131 072 34 / 64,
+  //             1024 x 131 072 391 / 338
+  if (workspace && (with_top_p || (V > 32768 && (!with_min_p || rows <= 128))))
+    return launch_slices<T>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, workspace, s);
+  const bool filter = set.top_k || with_top_p || with_min_p || (set.top_k_value > 0 && set.top_k_value < V);
   return filter ? launch_sample<T, true>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, s)
                 : launch_sample<T, false>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, s);
 }
@@ -1614,7 +1634,7 @@ using namespace ot;
 extern "C" {
 
 size_t ot_sample_symbols_workspace_bytes(int64_t rows, int32_t V, int32_t with_top_k) {
-  if (rows <= 0 || V <= 16384 || V > kMostSlices * kSlice || with_top_k) return 0;
+  if (rows <= 0 || V <= kLongRow || V > kMostSlices * kSlice || with_top_k) return 0;
   return (size_t)(rows < kSliceRows ? rows : kSliceRows) * slice_row_bytes(V);
 }
 

@@ -265,6 +265,44 @@ def test_sample_many_rows(rows, V, device):
         _check_sample(x, u, **SETTINGS[s])
 
 
+@pytest.mark.parametrize("rows,V", [(300, 16400), (257, 50000), (3, 524288), (2, 524289), (129, 33000)])
+def test_sample_long_rows_in_batches(rows, V, device):
+    """More rows than slices are kept for at a time, the longest row that is cut into slices, the next one."""
+    rng = np.random.default_rng(rows)
+    x, u = _logits(rng, rows, V, "bf16", device, sigma=1.5)
+    for settings in ({}, {"top_p": 0.9}, {"min_p": 0.2}, {"temperature": 2.0, "top_p": 0.99, "min_p": 1e-3}):
+        _check_sample(x, u, **settings)
+
+
+@pytest.mark.parametrize("V", [20000, 70000])
+def test_sample_long_rows_of_few_values(V, device):
+    """Cuts inside thousands of equal values, next to rows of two values one rounding apart."""
+    rng = np.random.default_rng(V)
+    x = rng.integers(0, 3, (8, V)).astype(np.float32)
+    x[4:] = np.nextafter(np.float32(7), np.float32(8) * rng.integers(0, 2, (4, V)).astype(np.float32))
+    x[6, rng.random(V) < 0.9] = -np.inf
+    x[7] = -30.0
+    x[7, V - 3] = 5.0
+    x = torch.from_numpy(x).to(device)
+    u = torch.from_numpy(rng.random(8, dtype=np.float32)).to(device)
+    for p in (0.0, 1e-6, 0.3, 0.5, 0.9, 1.0 - 2.0 ** -24):
+        _check_sample(x, u, top_p=p)
+        _check_sample(x, u, top_p=p, temperature=1e-3)
+        _check_sample(x, u, top_p=p, temperature=1e6, min_p=0.999999)
+
+
+def test_sample_a_long_row_does_not_depend_on_its_neighbours(device):
+    rng = np.random.default_rng(8)
+    x, u = _logits(rng, 300, 20000, "f32", device)
+    for s in ({"top_p": 0.8}, {"top_p": 0.95, "min_p": 0.01, "temperature": 1.4}):
+        a, lp = ot.sample_symbols(x, u, **s)
+        for r in (0, 1, 255, 256, 299):
+            b, lq = ot.sample_symbols(x[r:r + 1], u[r:r + 1], **s)
+            assert int(b) == int(a[r]) and float(lq) == float(lp[r])
+        again, lq = ot.sample_symbols(x, u, **s)
+        assert torch.equal(a, again) and torch.equal(lp, lq)
+
+
 @pytest.mark.parametrize("V", [64, 500, 1100, 6000, 40000])
 def test_sample_ties(V, device):
     """Values on a coarse grid: the cuts of top_k and top_p fall inside runs of equal values."""
