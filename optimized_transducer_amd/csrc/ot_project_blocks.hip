@@ -24,7 +24,6 @@ namespace ot {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -35,7 +34,7 @@ constexpr int kSmallCols = 64;     // vocabulary entries of a workgroup of the s
 // the wide kernel: vocabulary entries of a stage, tiles of 16 rows of a wave, rows of a workgroup
 constexpr int kWideCols = 64, kWideTiles = 2, kWideRows = kWavesPerBlock * kWideTiles * 16;
 constexpr int kDeepCols = 128;     // the deep kernel: vocabulary entries of a workgroup
-constexpr int kPartCols = 16;      // least vocabulary entries behind one partial log-sum-exp
+constexpr int kPartCols = 64;      // least vocabulary entries behind one partial log-sum-exp
 
 // a running log-sum-exp as (largest value, sum of exp(value - largest))
 struct LogSum {
@@ -149,21 +148,6 @@ __global__ __launch_bounds__(kBlock) void project_blocks_small_kernel(
   }
 }
 
-// 4 consecutive logits of a row; the row may start anywhere its type can
-template <class T>
-__device__ __forceinline__ void store_logits4(void *logits, int64_t i, const float y[4]) {
-  if constexpr (sizeof(T) == 4) {
-    typedef f32x4 unaligned __attribute__((aligned(4)));
-    const f32x4 t = {y[0], y[1], y[2], y[3]};
-    *reinterpret_cast<unaligned *>(static_cast<float *>(logits) + i) = t;
-  } else {
-    typedef u32x2 unaligned __attribute__((aligned(2)));
-    const u32x2 t = {(unsigned)from_float<T>(y[0]) | ((unsigned)from_float<T>(y[1]) << 16),
-                     (unsigned)from_float<T>(y[2]) | ((unsigned)from_float<T>(y[3]) << 16)};
-    *reinterpret_cast<unaligned *>(static_cast<unsigned short *>(logits) + i) = t;
-  }
-}
-
 // Many rows of up to KB blocks.  A workgroup of 4 waves owns 128 packed rows; a wave holds its 32
 // rows of x, widened, in registers for the whole walk over the vocabulary, so x is read and widened
 // once.  The weight goes by in stages of 64 vocabulary entries (all of D, 8-bit, 32 KB at D = 512),
@@ -182,7 +166,9 @@ __device__ __forceinline__ void store_logits4(void *logits, int64_t i, const flo
 // Which entry of the vocabulary a row of the accumulator tile stands for is free: it is chosen so
 // that a lane ends up with 16 bytes of consecutive logits and four lanes with 64, from one group of
 // 16 entries for 4-byte logits and from two for 2-byte ones.
-//   ALIGNED: 16 bytes of logits start at a multiple of 4 bytes (else 2-byte logits one by one)
+//   ALIGNED: 16 bytes of logits start at a multiple of 4 bytes.  Else (2-byte logits of an odd V)
+//   they go through ordinary stores, which any element may start at, and not the buffer view's:
+//   100 000 x 512 x 501 float16 146 us with stores of single elements, 93 so
 // Lane l holds bytes [64 q + 16 (l / 16), + 16) of a block of row l % 16 (q = 0, 1); the first 8
 // feed matrix instruction 2 q and the others 2 q + 1, in both operands alike.
 template <class T, int KB, bool ALIGNED, bool DEN>
@@ -203,6 +189,8 @@ struct WideProject {
   bf16x8 x[kWideTiles][KB][4];
   const float (*xs)[16][kWideTiles];  // this wave's scales of x in LDS
   __amdgpu_buffer_rsrc_t out;
+  char *out_base;              // the same place
+  bool rows_in;                // all rows of this wave are there
   unsigned out_row, out_tile;  // byte offsets of this lane's first logit and from tile to tile
   float ref[kWideTiles], sum[kWideTiles];
   i32x4 raw[2][2];  // weight of a step and of the next one
@@ -337,12 +325,19 @@ struct WideProject {
 #pragma unroll
       for (int t = 0; t < kWideTiles; ++t) __builtin_amdgcn_raw_buffer_store_b128(four[t], out, to + t * out_tile, 0, 0);
     }
-    if (!ALIGNED || !whole) {
+    const bool single = v + kGroup > V;  // (those that there are of a group that V cuts)
+    if (!ALIGNED && rows_in) {
+      typedef u32x4 unaligned __attribute__((aligned(2)));
+      if (whole || !single)
+#pragma unroll
+        for (int t = 0; t < kWideTiles; ++t) *reinterpret_cast<unaligned *>(out_base + dst + t * out_tile) = four[t];
+    }
+    if (!whole || (!ALIGNED && !rows_in)) {
 #pragma unroll
       for (int t = 0; t < kWideTiles; ++t)
 #pragma unroll
         for (int i = 0; i < kGroup; ++i)
-          if (v + i < V && (!ALIGNED || v + kGroup > V)) {
+          if (v + i < V && (single || (!ALIGNED && !rows_in))) {
             if constexpr (kOut == 4)
               __builtin_amdgcn_raw_buffer_store_b32(four[t][i], out, dst + t * out_tile + 4 * i, 0, 0);
             else
@@ -449,7 +444,9 @@ __global__ __launch_bounds__(kBlock, 2) void project_blocks_wide_kernel(
         p.at[sub][q][odd] = row * P::kSlots + ((8 * odd + 4 * q + p.h) ^ P::swizzle(row));
       }
   // this workgroup's logits; rows past the end are dropped by the view's bounds
-  p.out = make_buffer(static_cast<char *>(logits) + group0 * V * P::kOut,
+  p.out_base = static_cast<char *>(logits) + group0 * V * P::kOut;
+  p.rows_in = row0 + 16 * kWideTiles <= rows;
+  p.out = make_buffer(p.out_base,
                       (unsigned)min((int64_t)kWideRows, rows - group0) * (unsigned)V * P::kOut);
   p.out_row = ((unsigned)(p.wave * (16 * kWideTiles) + p.r) * (unsigned)V + (unsigned)(P::kGroup * p.h)) * P::kOut;
   p.out_tile = 16u * (unsigned)V * P::kOut;
@@ -597,7 +594,9 @@ __global__ __launch_bounds__(kBlock, 2) void project_blocks_deep_kernel(
       const int row = E::entry(sub, r);
       p.e.at[sub][q][0] = row * 8 + ((4 * q + h) ^ E::swizzle(row));
     }
-  p.e.out = make_buffer(static_cast<char *>(logits) + group0 * V * E::kOut,
+  p.e.out_base = static_cast<char *>(logits) + group0 * V * E::kOut;
+  p.e.rows_in = row0 + 16 * kWideTiles <= rows;
+  p.e.out = make_buffer(p.e.out_base,
                         (unsigned)min((int64_t)kWideRows, rows - group0) * (unsigned)V * E::kOut);
   p.e.out_row = ((unsigned)(p.e.wave * (16 * kWideTiles) + r) * (unsigned)V + (unsigned)(E::kGroup * h)) * E::kOut;
   p.e.out_tile = 16u * (unsigned)V * E::kOut;
