@@ -33,7 +33,6 @@ constexpr int kBlocksUnit = 16;    // D is a multiple of this: one 16-byte load
 constexpr int kSmallCols = 64;     // vocabulary entries of a workgroup of the small kernel
 // the wide kernel: vocabulary entries of a stage, tiles of 16 rows of a wave, rows of a workgroup
 constexpr int kWideCols = 64, kWideTiles = 2, kWideRows = kWavesPerBlock * kWideTiles * 16;
-constexpr int kDeepCols = 128;     // the deep kernel: vocabulary entries of a workgroup
 constexpr int kPartCols = 64;      // least vocabulary entries behind one partial log-sum-exp
 
 // a running log-sum-exp as (largest value, sum of exp(value - largest))
@@ -463,17 +462,22 @@ __global__ __launch_bounds__(kBlock, 2) void project_blocks_wide_kernel(
   if constexpr (DEN) p.finish_den(row0, rows, part, gridDim.y, den, parts);
 }
 
-// Many rows of any length.  A workgroup of 4 waves forms 128 packed rows x 128 vocabulary entries,
-// a wave 32 x 128 in 64 running sums per lane, block of D after block: the weight's block goes
-// straight into one of two LDS buffers, a wave's block of x into registers, both one step ahead of
-// the 64 matrix instructions of a step.  The workgroups of one group of rows have ids 8 apart and
-// run on one XCD, whose L2 serves x to all but the first.
-template <class T, bool ALIGNED, bool DEN>
+// Many rows of any length.  A workgroup of 4 waves forms 128 packed rows x COLS vocabulary entries
+// (64 or 128), a wave 32 x COLS in COLS / 2 running sums per lane, block of D after block: the
+// weight's block goes straight into one of two LDS buffers, a wave's block of x into registers, both
+// one step ahead of the COLS / 2 matrix instructions of a step (two steps ahead spilled registers and
+// took 37 us where one takes 32).  Each XCD has an eighth of the tiles in order, so that its L2
+// serves x to all but the first tile of a group of rows.
+//
+// The matrix instructions, the widening in front of them and the LDS reads of a step follow each
+// other within a wave and overlap between the two or three of a SIMD: 30 000 x 4096 x 500 float32
+// logits take 170 us, 723 TFLOP/s, of the 1380 that a large bfloat16 product reaches.
+template <class T, int COLS, bool ALIGNED, bool DEN>
 struct DeepProject {
   typedef WideProject<T, 1, ALIGNED, DEN> Wide;  // one block: layout of a step, epilogue
   static constexpr int kSubs = Wide::kSubs;
-  static constexpr int kGroups = kDeepCols / 16;
-  typedef i32x4 Weights[kDeepCols * 8];
+  static constexpr int kGroups = COLS / 16;
+  typedef i32x4 Weights[COLS * 8];
 
   Wide e;
   const unsigned char *x[kWideTiles];  // this lane's rows
@@ -484,11 +488,11 @@ struct DeepProject {
   float raw_scale[kWideTiles];
 
   __device__ __forceinline__ void load(int b, i32x4 *weights) {
-    const int n = min(kDeepCols, e.V - v0);
+    const int n = min(COLS, e.V - v0);
     const __amdgpu_buffer_rsrc_t from = make_buffer(e.w + (int64_t)v0 * e.D, (unsigned)n * (unsigned)e.D);
 #pragma unroll
-    for (int i = 0; i < kDeepCols * 8 / kBlock; ++i) {
-      const int first = (e.wave * (kDeepCols * 8 / kBlock) + i) * kWave, p = first + e.lane;
+    for (int i = 0; i < COLS * 8 / kBlock; ++i) {
+      const int first = (e.wave * (COLS * 8 / kBlock) + i) * kWave, p = first + e.lane;
       const int row = p / 8, k = b * kBlocksK + 16 * ((p % 8) ^ Wide::swizzle(row));
       const unsigned src = k < e.D ? (unsigned)row * (unsigned)e.D + (unsigned)k : 0xfffffff0u;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)(weights + first), 16,
@@ -544,19 +548,21 @@ struct DeepProject {
   }
 };
 
-template <class T, bool ALIGNED, bool DEN>
-__global__ __launch_bounds__(kBlock, 2) void project_blocks_deep_kernel(
+template <class T, int COLS, bool ALIGNED, bool DEN>
+__global__ __launch_bounds__(kBlock, COLS == 64 ? 3 : 2) void project_blocks_deep_kernel(
     const unsigned char *__restrict__ x, const float *__restrict__ xs, const unsigned char *__restrict__ w,
     const float *__restrict__ ws, const float *__restrict__ bias, int64_t rows, int D, int V, int chunks,
     void *__restrict__ logits, float *__restrict__ den, LogSum *__restrict__ parts) {
-  typedef DeepProject<T, ALIGNED, DEN> P;
+  typedef DeepProject<T, COLS, ALIGNED, DEN> P;
   typedef typename P::Wide E;
   __shared__ __attribute__((aligned(16))) typename P::Weights s_w0, s_w1;
   const int64_t id = (int64_t)blockIdx.z * gridDim.x + blockIdx.x;
-  const int64_t k = id >> 3;
-  const int64_t group0 = (k / chunks * 8 + (id & 7)) * kWideRows;
-  if (group0 >= rows) return;
-  const int chunk = (int)(k % chunks);
+  // an eighth of the tiles for each XCD, in order: chunk by chunk of a group of rows
+  const int64_t tiles = (rows + kWideRows - 1) / kWideRows * chunks, share = (tiles + 7) / 8;
+  const int64_t tile = (id & 7) * share + (id >> 3);
+  if ((id >> 3) >= share || tile >= tiles) return;
+  const int64_t group0 = tile / chunks * kWideRows;
+  const int chunk = (int)(tile % chunks);
   P p;
   p.e.w = w;
   p.e.ws = ws;
@@ -565,7 +571,7 @@ __global__ __launch_bounds__(kBlock, 2) void project_blocks_deep_kernel(
   p.e.lane = threadIdx.x & 63;
   p.e.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = p.e.r = p.e.lane & 15, h = p.e.h = p.e.lane >> 4;
-  p.v0 = chunk * kDeepCols;
+  p.v0 = chunk * COLS;
   p.nblocks = (D + kBlocksK - 1) / kBlocksK;
   const int64_t row0 = group0 + p.e.wave * (16 * kWideTiles);
 #pragma unroll
@@ -683,22 +689,22 @@ static int launch_project_blocks_wide(const unsigned char *x, const float *xs, c
   return (int)hipGetLastError();
 }
 
-template <class T>
+template <class T, int COLS>
 static int launch_project_blocks_deep(const unsigned char *x, const float *xs, const unsigned char *w,
                                       const float *ws, const float *bias, int64_t rows, int32_t D, int32_t V,
                                       void *logits, float *den, LogSum *parts, hipStream_t s) {
-  const int chunks = (V + kDeepCols - 1) / kDeepCols;
-  const int64_t row_groups = (rows + kWideRows - 1) / kWideRows, groups = (row_groups + 7) / 8 * 8 * chunks;
+  const int chunks = (V + COLS - 1) / COLS;
+  const int64_t tiles = (rows + kWideRows - 1) / kWideRows * chunks, groups = (tiles + 7) / 8 * 8;
   // (a launch holds 2^32 threads at most in each direction; a multiple of 8 keeps the ids' order)
   constexpr int64_t kMostX = 1 << 20;
   const dim3 grid((unsigned)(groups < kMostX ? groups : kMostX), 1, (unsigned)((groups + kMostX - 1) / kMostX));
   const bool merged = den && chunks > 1;
 #define OT_DEEP(ALIGNED_)                                                                                     \
   if (den)                                                                                                    \
-    hipLaunchKernelGGL((project_blocks_deep_kernel<T, ALIGNED_, true>), grid, dim3(kBlock), 0, s, x, xs, w, ws, \
+    hipLaunchKernelGGL((project_blocks_deep_kernel<T, COLS, ALIGNED_, true>), grid, dim3(kBlock), 0, s, x, xs, w, ws, \
                        bias, rows, D, V, chunks, logits, merged ? nullptr : den, merged ? parts : nullptr);   \
   else                                                                                                        \
-    hipLaunchKernelGGL((project_blocks_deep_kernel<T, ALIGNED_, false>), grid, dim3(kBlock), 0, s, x, xs, w,  \
+    hipLaunchKernelGGL((project_blocks_deep_kernel<T, COLS, ALIGNED_, false>), grid, dim3(kBlock), 0, s, x, xs, w,  \
                        ws, bias, rows, D, V, chunks, logits, (float *)nullptr, (LogSum *)nullptr)
   if (sizeof(T) == 4 || (V % 2 == 0 && (reinterpret_cast<uintptr_t>(logits) & 3) == 0)) {
     OT_DEEP(true);
@@ -738,7 +744,14 @@ static int launch_project_blocks(const unsigned char *x, const float *xs, const 
     if (nblocks == 3) OT_PROJECT_WIDE(3);
     if (nblocks == 4) OT_PROJECT_WIDE(4);
 #undef OT_PROJECT_WIDE
-    return launch_project_blocks_deep<T>(x, xs, w, ws, bias, rows, D, V, logits, den, parts, s);
+    // 64 entries a workgroup where 128 would give fewer than two rounds on every compute unit: us with
+    // 64 and 128, by the workgroups of 128 entries: 2100 x 640 x 1001 (136) 16 and 18, 600 x 1536 x
+    // 8000 (315) 42 and 43, 1003 x 1008 x 4998 (320) 32 and 36; 8000 x 2048 x 5000 (2520) 278 and 214,
+    // 30 000 x 4096 x 500 (940) 211 and 164
+    const int64_t groups = (rows + kWideRows - 1) / kWideRows * ((V + 127) / 128);
+    return groups < 2 * (int64_t)cus
+               ? launch_project_blocks_deep<T, 64>(x, xs, w, ws, bias, rows, D, V, logits, den, parts, s)
+               : launch_project_blocks_deep<T, 128>(x, xs, w, ws, bias, rows, D, V, logits, den, parts, s);
   }
   const dim3 grid((unsigned)(tiles < (1 << 22) ? tiles : (1 << 22)));
   hipLaunchKernelGGL((project_blocks_small_kernel<T>), grid, dim3(kBlock), 0, s, x, xs, w, ws, bias, rows, D,

@@ -139,7 +139,9 @@ SHAPES = [(1, 16, 1), (1, 128, 64), (2, 144, 5), (15, 64, 17), (16, 512, 500), (
           # each kernel at its smallest and odd sizes: blocks 1 to 4, then longer rows
           (13000, 16, 33), (13000, 128, 65), (6600, 240, 127), (3300, 256, 250), (3301, 384, 251), (3333, 400, 129),
           (1700, 512, 1021), (1700, 496, 1022), (6500, 1040, 257), (2111, 640, 1001), (5000, 2064, 130),
-          (700, 1536 + 16, 3001)]
+          (700, 1536 + 16, 3001),
+          # enough tiles of 128 x 128 for the longer rows
+          (9000, 1040, 1025), (16500, 640, 514), (2000, 528, 4997)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
