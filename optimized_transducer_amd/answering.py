@@ -85,7 +85,8 @@ def sample_symbols(logits: torch.Tensor, uniform: torch.Tensor,
     times the sum of all of them (the first always remains); of those, the entries with
     w_i >= ``min_p``.  The symbol is the first index, in index order, whose running sum of
     remaining weights exceeds ``uniform`` times their total.  Weights and sums behave as in
-    64 bits, so the symbol does not depend on the shape of the launch.
+    64 bits: only where a border lies within a rounding of those can the symbol depend on how
+    many rows are drawn from at once.
 
     Args:
       logits: (rows, V) float32, float16 or bfloat16 on a HIP device; any row pitch (columns

@@ -85,9 +85,11 @@ __device__ __forceinline__ i32x8 load_k32(const unsigned char *row, int k0, int 
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// A workgroup of 4 waves forms 16 packed rows x 64 vocabulary entries, a wave one
+// Few rows.  A workgroup of 4 waves forms 16 packed rows x 64 vocabulary entries, a wave one
 // accumulator tile of 16 x 16 straight from memory.  Lane l holds elements
-// [32 * (l / 16), + 32) of a block of row l % 16 of either operand.
+// [32 * (l / 16), + 32) of a block of row l % 16 of either operand.  The loads' latency, block
+// after block, is what it waits for: 1 x 1024 x 16384 takes 8.1 us, 2.1 TB/s of weight, where a
+// launch alone is 5.
 template <class T>
 __global__ __launch_bounds__(kBlock) void project_blocks_small_kernel(
     const unsigned char *__restrict__ x, const float *__restrict__ xs, const unsigned char *__restrict__ w,
@@ -168,6 +170,10 @@ __global__ __launch_bounds__(kBlock) void project_blocks_small_kernel(
 //   ALIGNED: 16 bytes of logits start at a multiple of 4 bytes.  Else (2-byte logits of an odd V)
 //   they go through ordinary stores, which any element may start at, and not the buffer view's:
 //   100 000 x 512 x 501 float16 146 us with stores of single elements, 93 so
+// What bounds it: the stores of the logits, in partial lines where V * the size of a logit is no
+// multiple of 128 bytes, and behind them the matrix instructions.  751 992 x 512 x 500 bfloat16 with
+// denominators 0.53 ms, 725 TFLOP/s and 2.2 TB/s; 149 346 x 512 x 5000 float32 1.24 ms, 619 TFLOP/s
+// and 2.5 TB/s (tiles straight from memory, as the small kernel's: 3.19 and 6.26 ms).
 // Lane l holds bytes [64 q + 16 (l / 16), + 16) of a block of row l % 16 (q = 0, 1); the first 8
 // feed matrix instruction 2 q and the others 2 q + 1, in both operands alike.
 template <class T, int KB, bool ALIGNED, bool DEN>
@@ -730,11 +736,13 @@ static int launch_project_blocks(const unsigned char *x, const float *xs, const 
   // The small kernel spreads over the chip what the others would do on a few compute units, but
   // reads its operands again for every 16 x 64 logits.  Microseconds with denominators, small
   // against wide or deep, by its workgroups (256 compute units):
-  //   D = 512:  32 x 5000 (158) 10 : 12, 64 x 5000 (316) 12 : 12, 512 x 500 (256) 9 : 11,
-  //             1024 x 500 (512) 12 : 11, 128 x 5000 (632) 15 : 13
-  //   D = 1008: 256 x 5000 (1264) 26 : 31, 512 x 5000 (2528) 44 : 31
-  //   D = 2048: 512 x 500 (256) 16 : 32, 1024 x 500 (512) 26 : 32, 4096 x 500 (2048) 88 : 33
-  const bool few = nblocks <= 4 ? 2 * tiles <= 3 * (int64_t)cus : tiles * nblocks <= 40 * (int64_t)cus;
+  //   D = 512:  32 x 5000 (158) 11 : 13, 512 x 500 (256) 10 : 12, 64 x 5000 (316) 14 : 13,
+  //             1024 x 500 (512) 13 : 12, 128 x 5000 (632) 16 : 14
+  //   D = 1008: 32 x 5000 (158) 12 : 15, 64 x 5000 (316) 14 : 16, 768 x 500 (384) 13 : 15,
+  //             128 x 5000 (632) 20 : 16, 512 x 5000 (2528) 46 : 22;  D = 1024: 32 x 16384 (512) 24 : 21
+  //   D = 2048: 32 x 5000 (158) 19 : 22, 512 x 500 (256) 17 : 25, 64 x 5000 (316) 28 : 22,
+  //             640 x 500 (320) 26 : 25, 4096 x 500 (2048) 90 : 27;  D = 4096: 512 x 500 (256) 26 : 43
+  const bool few = 2 * tiles <= (nblocks <= 8 ? 3 : 2) * (int64_t)cus;
   // (wide and deep address a workgroup's logits, and deep its weights, with 32 bits)
   if (!few && V < (1 << 21) && D < (1 << 24)) {
 #define OT_PROJECT_WIDE(KB_) \
