@@ -955,7 +955,7 @@ std::pair<torch::Tensor, torch::Tensor> sample_symbols(
   const int dtype = element_dtype(logits_in, "sample_symbols: logits");
   TORCH_CHECK(logits_in.is_cuda(), "sample_symbols: logits must be on a HIP device");
   TORCH_CHECK(logits_in.dim() == 2 && logits_in.size(1) > 0 && logits_in.size(0) <= INT32_MAX &&
-                  logits_in.size(1) <= INT32_MAX - 4096,
+                  logits_in.size(1) <= INT32_MAX - 8192,
               "sample_symbols: logits must have shape (rows, V) with V > 0, got ", logits_in.sizes());
   const int64_t rows = logits_in.size(0), V = logits_in.size(1);
   TORCH_CHECK(uniform_in.dim() == 1 && uniform_in.size(0) == rows && uniform_in.scalar_type() == torch::kFloat &&

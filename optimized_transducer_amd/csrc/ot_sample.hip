@@ -1645,7 +1645,7 @@ int ot_sample_symbols(const void *logits, int32_t dtype, int64_t row_stride, int
                       void *stream) {
   if (rows == 0) return 0;
   if (!logits || !uniform || !symbols || !log_probs || rows < 0 || rows > INT32_MAX || V <= 0 ||
-      V > INT32_MAX - 4096 || row_stride < 0)
+      V > INT32_MAX - 8192 || row_stride < 0)  // (indices of whole steps of 16 waves stay below 2^31)
     return OT_E_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(logits) & (dtype == OT_DTYPE_F32 ? 3 : 1)) ||
       (reinterpret_cast<uintptr_t>(uniform) & 3) || (reinterpret_cast<uintptr_t>(temperature) & 3) ||

@@ -117,9 +117,9 @@ def test_c_abi_refuses_bad_arguments():
     assert need(i64(0), i32(5)) == 0 and need(i64(5), i32(0)) == 0 and need(i64(5), i32(500)) > 0
 
     def sample(logits=one, dtype=0, stride=10, rows=4, V=10, uniform=one, t=null, k=null, p=null, m=null,
-               symbols=one, log_probs=one):
+               symbols=one, log_probs=one, work=null, work_bytes=0):
         return L.ot_sample_symbols(logits, i32(dtype), i64(stride), i64(rows), i32(V), uniform, t, f32(1), k,
-                                   i32(0), p, f32(1), m, f32(0), symbols, log_probs, null, size(0), null)
+                                   i32(0), p, f32(1), m, f32(0), symbols, log_probs, work, size(work_bytes), null)
 
     assert sample(rows=0) == 0
     L.ot_sample_symbols_workspace_bytes.restype = size
@@ -130,6 +130,9 @@ def test_c_abi_refuses_bad_arguments():
     for bad in (dict(logits=null), dict(uniform=null), dict(symbols=null), dict(log_probs=null), dict(rows=-1),
                 dict(rows=1 << 31), dict(V=0), dict(V=2 ** 31 - 1), dict(stride=-1), dict(dtype=5)):
         assert sample(**bad) == -1, bad
+    # the indices of a step of 16 waves x 64 lanes x 8 elements past the end stay below 2^31
+    assert sample(V=2 ** 31 - 8192) == -1 and sample(dtype=1, V=2 ** 31 - 4097) == -1
+    assert sample(V=50000, work=odd, work_bytes=1 << 24) == -3
     for bad in (dict(logits=odd), dict(logits=ctypes.c_void_p(66)), dict(uniform=odd), dict(t=odd), dict(k=odd),
                 dict(p=odd), dict(m=odd), dict(symbols=odd), dict(log_probs=odd)):
         assert sample(**bad) == -3, bad

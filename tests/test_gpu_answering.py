@@ -583,6 +583,47 @@ def test_chain_replays_from_a_hip_graph(device):
         torch.rand(1000, device=device).sum().item()
 
 
+def test_sample_long_rows_replay_and_overlap(device):
+    """Rows that several workgroups share: two graphs, and calls on two streams at once, do not share anything."""
+    rows, V = 70, 60000
+    x, u = torch.empty((rows, V), device=device), torch.empty(rows, device=device)
+    draw = lambda x, u: ot.sample_symbols(x, u, temperature=0.9, top_p=0.9, min_p=1e-4)  # noqa: E731
+    x.normal_()
+    u.uniform_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        draw(x, u)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(draw(x, u))
+        graphs.append(g)
+    for i in range(6):
+        x.normal_()
+        u.uniform_()
+        want = draw(x, u)
+        graphs[i % 2].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i % 2][0], want[0]) and torch.equal(outs[i % 2][1], want[1])
+        torch.rand(1000, device=device).sum().item()
+    inputs = [(torch.randn((rows, V), device=device) * 2, torch.rand(rows, device=device)) for _ in range(2)]
+    want = [draw(*i) for i in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(draw(*inputs[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for a in got[k]:
+            assert torch.equal(a[0], want[k][0]) and torch.equal(a[1], want[k][1])
+
+
 def test_offsets_beyond_32_bits(device):
     """More than 2^32 elements of logits: the last rows are the rows of a small call."""
     rows, V = 70001, 65536  # 4.6e9 elements, 9.2 GB of bfloat16
