@@ -94,6 +94,94 @@ __device__ __forceinline__ N wave_scan(N v) {
 __device__ __forceinline__ double wave_sum(double v) { return lane_value(wave_scan(v), kWave - 1); }
 __device__ __forceinline__ int wave_sum(int v) { return lane_value(wave_scan(v), kWave - 1); }
 
+// the value of lane ^ X, X = 2^n - 1 or 2^n
+template <int CTRL>
+__device__ __forceinline__ float dpp_value(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <int X>
+__device__ __forceinline__ float lane_xor(float v) {
+  if constexpr (X == 1) return dpp_value<kDppQuadXor1>(v);
+  else if constexpr (X == 2) return dpp_value<kDppQuadXor2>(v);
+  else if constexpr (X == 3) return dpp_value<0x1b>(v);                       // quad_perm 3 2 1 0
+  else if constexpr (X == 4) return dpp_value<0x1b>(dpp_value<kDppRowHalfMirror>(v));
+  else if constexpr (X == 7) return dpp_value<kDppRowHalfMirror>(v);
+  else if constexpr (X == 8) return dpp_value<0x128>(v);                      // row_ror 8
+  else if constexpr (X == 15) return dpp_value<kDppRowMirror>(v);
+  else return __shfl_xor(v, X, kWave);
+}
+
+// Sorts the 64 * N values of a wave, larger ones first; value i of lane l ends as number l * N + i.
+// A bitonic network whose merges start by comparing a block with its mirror image, so that the lower
+// place always takes the larger value: within a lane a maximum and a minimum, between lanes the
+// median of the two values and an infinity of the lane's side.
+template <int N>
+__device__ __forceinline__ void sort_in_lane(float (&v)[N], int stride) {
+#pragma unroll
+  for (int d = stride; d > 0; d /= 2)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (!(i & d)) {
+        const float a = v[i], b = v[i | d];
+        v[i] = fmaxf(a, b);
+        v[i | d] = fminf(a, b);
+      }
+}
+template <int X, int N>
+__device__ __forceinline__ void sort_lanes(float (&v)[N], int lane, bool mirror) {
+  // (lower half of the compared pair: the bit of the lane that X's highest one is)
+  constexpr int kTop = X & ~(X >> 1);
+  const float side = lane & kTop ? OT_NEG_INF : kInf;
+  float other[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) other[i] = lane_xor<X>(v[mirror ? N - 1 - i : i]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = __builtin_amdgcn_fmed3f(v[i], other[i], side);
+}
+template <int N>
+__device__ __forceinline__ void wave_sort(float (&v)[N], int lane) {
+#pragma unroll
+  for (int size = 2; size <= N; size *= 2) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int j = i ^ (size - 1);
+      if (i < j) {
+        const float a = v[i], b = v[j];
+        v[i] = fmaxf(a, b);
+        v[j] = fminf(a, b);
+      }
+    }
+    sort_in_lane(v, size / 4);
+  }
+  sort_lanes<1>(v, lane, true);
+  sort_in_lane(v, N / 2);
+  sort_lanes<3>(v, lane, true);
+  sort_lanes<1>(v, lane, false);
+  sort_in_lane(v, N / 2);
+  sort_lanes<7>(v, lane, true);
+  sort_lanes<2>(v, lane, false);
+  sort_lanes<1>(v, lane, false);
+  sort_in_lane(v, N / 2);
+  sort_lanes<15>(v, lane, true);
+  sort_lanes<4>(v, lane, false);
+  sort_lanes<2>(v, lane, false);
+  sort_lanes<1>(v, lane, false);
+  sort_in_lane(v, N / 2);
+  sort_lanes<31>(v, lane, true);
+  sort_lanes<8>(v, lane, false);
+  sort_lanes<4>(v, lane, false);
+  sort_lanes<2>(v, lane, false);
+  sort_lanes<1>(v, lane, false);
+  sort_in_lane(v, N / 2);
+  sort_lanes<63>(v, lane, true);
+  sort_lanes<16>(v, lane, false);
+  sort_lanes<8>(v, lane, false);
+  sort_lanes<4>(v, lane, false);
+  sort_lanes<2>(v, lane, false);
+  sort_lanes<1>(v, lane, false);
+  sort_in_lane(v, N / 2);
+}
+
 // ---- the threads that share a row -----------------------------------------------------------
 
 template <int WAVES>
@@ -602,10 +690,61 @@ struct Sampler {
 
   // the cuts; before them `lowest` is the smallest finite entry, of `finite` ones
   __device__ __forceinline__ void cut(int top_k, float top_p, float min_p, float lowest, int finite) {
-    if (top_k > 0 && top_k < V) keep_top_k(top_k, lowest, finite);
-    weigh();
-    if (top_p < 1.f) keep_top_p(fmaxf(top_p, 0.f), lowest);
+    if constexpr (WAVES == 1) {
+      const int k = top_k > 0 ? min(top_k, finite) : finite;
+      if (k < finite || top_p < 1.f) cut_sorted(k, top_p, finite);
+      weigh();
+    } else {
+      if (top_k > 0 && top_k < V) keep_top_k(top_k, lowest, finite);
+      weigh();
+      if (top_p < 1.f) keep_top_p(fmaxf(top_p, 0.f), lowest);
+    }
     if (min_p > 0.f) keep_min_p(fminf(min_p, 1.f));
+  }
+  // top_k and top_p by a wave that holds the row: the entries in order
+  __device__ __forceinline__ void cut_sorted(int k, float top_p, int finite) {
+    constexpr int N = CHUNKS * VEC;
+    float y[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = x[i / VEC][i % VEC];
+    wave_sort(y, g.lane);
+    int n = k;  // entries that remain
+    if (top_p < 1.f) {
+      double t[N], mine = 0.0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        t[i] = g.lane * N + i < k ? weight(y[i]) : 0.0;
+        mine += t[i];
+      }
+      const double upto = wave_scan(mine), want = fmax((double)top_p, 0.0) * lane_value(upto, kWave - 1);
+      double before = upto - mine;
+      int fit = 0;  // of this lane's entries, in front of the first that does not remain
+      bool all = true;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        all = all && (before < want || g.lane * N + i == 0);
+        fit += all;
+        before += t[i];
+      }
+      const uint64_t end = __ballot(fit < N);
+      if (end) {
+        const int l = __builtin_ctzll(end);
+        n = min(n, l * N + lane_value(fit, l));
+      }
+    }
+    if (n >= finite) return;
+    const int l = (n - 1) / N, i = (n - 1) % N;
+    float at = OT_NEG_INF;  // (a maximum, and not a choice between elements, which would index the registers)
+#pragma unroll
+    for (int e = 0; e < N; ++e) at = fmaxf(at, e == i ? y[e] : OT_NEG_INF);
+    const float v = lane_value(at, l);
+    int above = 0, at_v = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      above += __popcll(__ballot(y[e] > v));
+      at_v += __popcll(__ballot(y[e] == v));
+    }
+    exclude(v, n - above, at_v);
   }
   __device__ __forceinline__ void weigh() {
     if constexpr (kHeldWeights) {
@@ -670,6 +809,13 @@ struct Sampler {
   // `start`, `whole`: what lies in front of these entries and the total, where they are a slice of
   // a row
   __device__ __forceinline__ Drawn draw(double u, double start = 0.0, double whole = -1.0) {
+    if constexpr (WAVES == 1) {
+      int symbol;
+      float logit;
+      double total;
+      draw_alone(u, symbol, logit, total);
+      return {symbol, log_probability(logit, m, T_, total)};
+    }
     // totals of the waves' parts, then the part, the chunk, the lane and the element in which
     // the running sum passes u * total
     if (!part_known) {
