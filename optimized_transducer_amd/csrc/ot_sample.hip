@@ -186,7 +186,9 @@ __device__ __forceinline__ void wave_sort(float (&v)[N], int lane) {
 
 template <int WAVES>
 struct SampleShared {
-  unsigned bins[kSampleBins];
+  // (one wave that holds its row sorts it instead)
+  unsigned bins[WAVES > 1 ? kSampleBins : 1];
+  float few[WAVES > 1 ? kSampleFew : 1];  // entries of one bin
   double sum[WAVES];
   float value[2][WAVES];
   int count[WAVES];
@@ -622,10 +624,153 @@ struct Sampler {
     g.gather(part, part_at, sum, at_v);
   }
 
+  // Of `count` entries in s.few, in front of which weights of `above` lie: how many remain for
+  // `want`; the last of them, n of the at_v entries at its value.  False if the border is not among
+  // them.
+  template <int N>
+  __device__ __forceinline__ bool settle(int count, double above, double want, float &v, int &n, int &at_v) const {
+    float y[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = g.lane * N + i < count ? g.s.few[g.lane * N + i] : OT_NEG_INF;
+    wave_sort(y, g.lane);
+    if (sorted_fit(y, count, above, [&](double) { return want; }, n) < want && n == count) return false;
+    if (n == 0) return false;
+    v = sorted_value(y, n - 1);
+    int over = 0;
+    at_v = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      over += __popcll(__ballot(y[e] > v));
+      at_v += __popcll(__ballot(y[e] == v));
+    }
+    n -= over;
+    return true;
+  }
+  // The first k of a wave's sorted entries, weights of `above` in front of them: returns the sum of
+  // both, and in n how many of the entries have less than want(that sum) in front of them (the row's
+  // largest entry counts anyway).
+  template <int N, class W>
+  __device__ __forceinline__ double sorted_fit(const float (&y)[N], int k, double above, W want_of, int &n) const {
+    double t[N], mine = 0.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      t[i] = g.lane * N + i < k ? weight(y[i]) : 0.0;
+      mine += t[i];
+    }
+    const double upto = wave_scan(mine), total = above + lane_value(upto, kWave - 1), want = want_of(total);
+    double before = above + (upto - mine);
+    int fit = 0;  // of this lane's entries, in front of the first that does not remain
+    bool all = true;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      all = all && (before < want || (g.lane * N + i == 0 && y[i] == m));
+      fit += all;
+      before += t[i];
+    }
+    n = k;
+    const uint64_t end = __ballot(fit < N);
+    if (end) {
+      const int l = __builtin_ctzll(end);
+      n = min(k, l * N + lane_value(fit, l));
+    }
+    return total;
+  }
+  // entry number `at` of a wave's sorted ones
+  template <int N>
+  __device__ __forceinline__ static float sorted_value(const float (&y)[N], int at) {
+    float v = OT_NEG_INF;  // (a maximum, and not a choice between elements, which would index the registers)
+#pragma unroll
+    for (int e = 0; e < N; ++e) v = fmaxf(v, e == at % N ? y[e] : OT_NEG_INF);
+    return lane_value(v, at / N);
+  }
+
+  // top_p's cut where it falls into one bin of few entries: their order settles it.  False if it
+  // does not; the bins' 32-bit sums, in whatever order they are formed, decide about no more than
+  // that.
+  __device__ __forceinline__ bool cut_in_one_bin(double want, float from) {
+    float *const bin_weight = reinterpret_cast<float *>(g.s.bins);
+    const float half = 0.5f * m - 0.5f * from;
+    if (!(half > 1e-30f)) return false;
+    const float per_unit = (0.5f * kSampleBins) / half;
+    auto bin = [&](float y) -> int { return (int)fminf((m - y) * per_unit, kSampleBins - 1.0f); };
+    for (int i = g.thread(); i < kSampleBins; i += WAVES * kWave) bin_weight[i] = 0.f;
+    if (g.thread() == 0) g.s.index = 0;
+    g.sync();
+    const float per_octave = (float)weight.c;
+    each([&](int, int, const float *y) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (y[e] >= from) unsafeAtomicAdd(&bin_weight[bin(y[e])], __builtin_amdgcn_exp2f((y[e] - m) * per_octave));
+    });
+    g.sync();
+    // every wave looks for the bin: lane l holds bins [4 l, 4 l + 4)
+    constexpr int kPer = kSampleBins / kWave;
+    double amount[kPer], mine = 0.0;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+      amount[q] = (double)bin_weight[g.lane * kPer + q];
+      mine += amount[q];
+    }
+    double run = wave_scan(mine) - mine;
+    int reached = kSampleBins;
+#pragma unroll
+    for (int q = kPer - 1; q >= 0; --q) {
+      double upto = run;
+#pragma unroll
+      for (int k = 0; k <= q; ++k) upto += amount[k];
+      if (amount[q] > 0.0 && upto >= want) reached = g.lane * kPer + q;
+    }
+    const uint64_t r = __ballot(reached < kSampleBins);
+    if (!r) {
+      g.sync();  // the bins have been read
+      return false;
+    }
+    const int pick = lane_value(reached, __builtin_ctzll(r));
+    double above = 0.0;
+    each([&](int j, int, const float *y) {
+      double t[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int b = y[e] >= from ? bin(y[e]) : kSampleBins;
+        t[e] = b < pick ? weight_of(j, e, y[e]) : 0.0;
+        if (b == pick) {
+          const int to = atomicAdd(&g.s.index, 1);
+          if (to < kSampleFew) g.s.few[to] = y[e];
+        }
+      }
+      above += pairwise(t);
+    });
+    int none = 0;
+    g.totals(above, none);  // (barriers: the entries are in place)
+    const int count = g.s.index;
+    if (count > kSampleFew) return false;
+    g.sync();  // the count has been read
+    if (g.wave == 0) {
+      float v = 0.f;
+      int n = 0, at_v = 0;
+      const bool ok = count <= kWave ? settle<1>(count, above, want, v, n, at_v)
+                                     : settle<kSampleFew / kWave>(count, above, want, v, n, at_v);
+      if (g.lane == 0) {
+        g.s.value[0][0] = v;
+        g.s.count[0] = n;
+        g.s.count[1] = at_v;
+        g.s.index = ok;
+      }
+    }
+    g.sync();
+    const bool ok = g.s.index;
+    const float v = g.s.value[0][0];
+    const int n = g.s.count[0], at_v = g.s.count[1];
+    g.sync();  // they have been read
+    if (ok) exclude(v, n, at_v);
+    return ok;
+  }
+
   __device__ __forceinline__ void keep_top_p(float p, float lowest) {
     double total;
     int none;
     sum_above<true>(lowest, total, none);
+    part_known = false;
     const double want = (double)p * total;
     // Entries of weights below (1 - p) * total / V come to less than what lies behind the cut.
     float from = lowest;
@@ -634,6 +779,7 @@ struct Sampler {
       const float z = __log2f((float)least_weight) / (float)weight.c;
       if (z > -1e30f) from = fminf(m, fmaxf(from, m + 1.001f * z));
     }
+    if (cut_in_one_bin(want, from)) return;
     double rough, sum;
     float v = select<true>(want, from, rough);
     int at_v, went = 0;
@@ -710,34 +856,11 @@ struct Sampler {
     wave_sort(y, g.lane);
     int n = k;  // entries that remain
     if (top_p < 1.f) {
-      double t[N], mine = 0.0;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        t[i] = g.lane * N + i < k ? weight(y[i]) : 0.0;
-        mine += t[i];
-      }
-      const double upto = wave_scan(mine), want = fmax((double)top_p, 0.0) * lane_value(upto, kWave - 1);
-      double before = upto - mine;
-      int fit = 0;  // of this lane's entries, in front of the first that does not remain
-      bool all = true;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        all = all && (before < want || g.lane * N + i == 0);
-        fit += all;
-        before += t[i];
-      }
-      const uint64_t end = __ballot(fit < N);
-      if (end) {
-        const int l = __builtin_ctzll(end);
-        n = min(n, l * N + lane_value(fit, l));
-      }
+      const double p = fmax((double)top_p, 0.0);
+      sorted_fit(y, k, 0.0, [&](double total) { return p * total; }, n);
     }
     if (n >= finite) return;
-    const int l = (n - 1) / N, i = (n - 1) % N;
-    float at = OT_NEG_INF;  // (a maximum, and not a choice between elements, which would index the registers)
-#pragma unroll
-    for (int e = 0; e < N; ++e) at = fmaxf(at, e == i ? y[e] : OT_NEG_INF);
-    const float v = lane_value(at, l);
+    const float v = sorted_value(y, n - 1);
     int above = 0, at_v = 0;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
@@ -815,89 +938,80 @@ struct Sampler {
       double total;
       draw_alone(u, symbol, logit, total);
       return {symbol, log_probability(logit, m, T_, total)};
-    }
-    // totals of the waves' parts, then the part, the chunk, the lane and the element in which
-    // the running sum passes u * total
-    if (!part_known) {
-      part = 0.0;
-      each([&](int j, int, const float *y) {
-        double t[VEC];
+    } else {
+      // totals of the waves' parts, then the part, the chunk, the lane and the element in which
+      // the running sum passes u * total
+      if (!part_known) {
+        part = 0.0;
+        each([&](int j, int, const float *y) {
+          double t[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) t[e] = weight_of(j, e, y[e]);
-        part += pairwise(t);
-      });
-      part = wave_sum(part);
-    }
-    double total = start + part, before = start;
-    if constexpr (WAVES > 1) {
+          for (int e = 0; e < VEC; ++e) t[e] = weight_of(j, e, y[e]);
+          part += pairwise(t);
+        });
+        part = wave_sum(part);
+      }
       g.sync();
       if (g.lane == 0) g.s.sum[g.wave] = part;
       if (g.thread() == 0) g.s.index = -1;
       g.sync();
-      total = start;
+      double total = start, before = start;
       for (int k = 0; k < WAVES; ++k) {
         if (k == g.wave) before = total;
         total += g.s.sum[k];
       }
-    }
-    if (whole >= 0.0) total = whole;
-    const double product = fmax(u, 0.0) * total;
-    const double target = product < total ? product : __builtin_huge_val();
-    int symbol = -1;
-    float logit = 0.f;
-    if (before <= target && target < before + part) {  // one wave
-      double run = before;
-      int last = -1;  // the wave's last entry with a weight
-      float last_logit = 0.f;
-      each([&](int j, int i, const float *y) {
-        if (symbol >= 0) return;
-        double t[VEC];
+      if (whole >= 0.0) total = whole;
+      const double product = fmax(u, 0.0) * total;
+      const double target = product < total ? product : __builtin_huge_val();
+      int symbol = -1;
+      float logit = 0.f;
+      if (before <= target && target < before + part) {  // one wave
+        double run = before;
+        int last = -1;  // the wave's last entry with a weight
+        float last_logit = 0.f;
+        each([&](int j, int i, const float *y) {
+          if (symbol >= 0) return;
+          double t[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) t[e] = weight_of(j, e, y[e]);
-        const double mine = pairwise(t), upto = wave_scan(mine);
-        const double chunk = lane_value(upto, kWave - 1);
-        const uint64_t pass = __ballot(run + upto > target);
-        const uint64_t some = __ballot(mine > 0.0);
-        if (some) {
-          find(t, y, i, run, mine, upto, target, pass, some, last, last_logit);
-          if (pass) symbol = last;
-        }
-        run += chunk;
-      });
-      logit = last_logit;
-      if (symbol < 0) symbol = last;
-      if constexpr (WAVES > 1) {
+          for (int e = 0; e < VEC; ++e) t[e] = weight_of(j, e, y[e]);
+          const double mine = pairwise(t), upto = wave_scan(mine);
+          const double chunk = lane_value(upto, kWave - 1);
+          const uint64_t pass = __ballot(run + upto > target);
+          const uint64_t some = __ballot(mine > 0.0);
+          if (some) {
+            find(t, y, i, run, mine, upto, target, pass, some, last, last_logit);
+            if (pass) symbol = last;
+          }
+          run += chunk;
+        });
+        logit = last_logit;
+        if (symbol < 0) symbol = last;
         if (g.lane == 0) {
           g.s.index = symbol;
           g.s.value[0][0] = logit;
         }
       }
-    }
-    if constexpr (WAVES > 1) {
       g.sync();
       symbol = g.s.index;
       logit = g.s.value[0][0];
-    }
-    if (symbol < 0) {  // u >= 1, or a product that rounds up to the total: the last entry with a weight
-      each([&](int j, int i, const float *y) {
-        int last = -1;
+      if (symbol < 0) {  // u >= 1, or a product that rounds up to the total: the last entry with a weight
+        each([&](int j, int i, const float *y) {
+          int last = -1;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (weight_of(j, e, y[e]) > 0.0) last = i + e;
-        const uint64_t some = __ballot(last >= 0);
-        if (some) symbol = lane_value(last, 63 - __builtin_clzll(some));
-      });
-      if constexpr (WAVES > 1) {
+          for (int e = 0; e < VEC; ++e)
+            if (weight_of(j, e, y[e]) > 0.0) last = i + e;
+          const uint64_t some = __ballot(last >= 0);
+          if (some) symbol = lane_value(last, 63 - __builtin_clzll(some));
+        });
         g.sync();
         if (g.lane == 0) g.s.count[g.wave] = symbol;
         g.sync();
         for (int k = 0; k < WAVES; ++k) symbol = max(symbol, g.s.count[k]);
+        logit = load_element<T>(row, symbol);
       }
-      logit = load_element<T>(row, symbol);
+      return {symbol, log_probability(logit, m, T_, total)};
     }
-    return {symbol, log_probability(logit, m, T_, total)};
   }
-
 };
 
 // What the cuts start from: the largest entry m, whether there is a NaN (bad < 0), the smallest
