@@ -18,8 +18,11 @@
 // polynomial for 2^f) where a 32-bit one through the hardware's 2^x costs 8 and the transcendental
 // unit.
 //
-// No sort: a cut is found by a histogram of the interval that still holds it, 256 bins at a
-// time, until one value is left; two levels do for rows without many equal values.
+// How the cuts are found: a wave that holds its row sorts it and reads both of them off the order
+// (32 x 512 float32, settings per row, 6.3 us, 11.7 by histograms).  Longer rows are not sorted: a
+// histogram of 256 bins finds the one that top_p's cut falls into, and only its entries are; for
+// top_k, and where such a bin holds too many, the interval that still holds the cut is divided
+// again, until one value is left or few enough entries are.
 //
 // Who works on a row (what bounds it; times at T = 1 and sigma 2):
 //   a wave                short rows, up to 512 (float32) or 1024 elements, in registers, and no
@@ -28,7 +31,7 @@
 //   4, 8 or 16 waves      rows up to 16384, in registers; of all the waves only the wide steps
 //                         profit, so that the barriers and scans of the cuts bound it.  A top_k of
 //                         512 at most is found by all of them, and one wave goes on with what is left
-//                         (20 011 x 5000 float16 with all cuts 0.46 ms, 0.72 with all waves to the end)
+//                         (20 011 x 5000 float16 with all cuts 0.41 ms, 0.94 with all waves to the end)
 //   slices                longer rows, several workgroups each (64 x 131 072 bfloat16, top_p: 69 us,
 //                         266 by a workgroup per row; launches and the chain of steps bound it)
 //   16 waves              rows beyond the slices, or with top_k: they read the row in every step,
@@ -779,7 +782,9 @@ struct Sampler {
       const float z = __log2f((float)least_weight) / (float)weight.c;
       if (z > -1e30f) from = fminf(m, fmaxf(from, m + 1.001f * z));
     }
-    if (cut_in_one_bin(want, from)) return;
+    // (rows of up to some hundred entries per bin: 64 x 50 000 float32 109 us, 138 without it;
+    // 64 x 131 072, where the bin holds too many, 512 and 337)
+    if (V <= kSampleBins * kSampleBins && cut_in_one_bin(want, from)) return;
     double rough, sum;
     float v = select<true>(want, from, rough);
     int at_v, went = 0;
@@ -1874,12 +1879,13 @@ static int launch_sample(const void *logits, int64_t row_stride, int64_t rows, i
                          hipStream_t s) {
   const bool with_top_p = set.top_p || set.top_p_value < 1.f, with_min_p = set.min_p || set.min_p_value > 0.f;
   // Slices or one workgroup of 16 waves (us, float32, slices first):
-  //   top_p     64 x 20 000 37 / 62, 4096 x 20 000 820 / 939, 64 x 131 072 69 / 337,
-  //             1024 x 131 072 656 / 1485; 64 x 16 000 (elements in registers) 35 / 40, 4096 732 / 646
-  //   no cuts   64 x 20 000 12 / 13, 4096 x 20 000 275 / 198, 64 x 50 000 14 / 26, 4096 x 50 000 425 / 469,
-  //             64 x 131 072 19 / 54
-  //   min_p     64 x 20 000 18 / 16, 64 x 50 000 23 / 31, 256 x 50 000 51 / 38, 64 x 131 072 34 / 64,
-  //             1024 x 131 072 391 / 338
+  //   top_p     64 x 20 000 36 / 50, 4096 x 20 000 815 / 782, 64 x 50 000 46 / 109, 4096 x 50 000
+  //             1350 / 1836, 64 x 131 072 70 / 337; 64 x 16 000 (elements in registers) 35 / 37,
+  //             4096 x 16 000 693 / 647
+  //   no cuts   64 x 20 000 12 / 13, 4096 x 20 000 276 / 197, 64 x 50 000 14 / 26, 4096 x 50 000 415 / 467,
+  //             64 x 131 072 20 / 55
+  //   min_p     64 x 20 000 19 / 16, 64 x 50 000 23 / 31, 256 x 50 000 51 / 37, 64 x 131 072 35 / 66,
+  //             1024 x 131 072 375 / 337
   if (workspace && (with_top_p || (V > 32768 && (!with_min_p || rows <= 128))))
     return launch_slices<T>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, workspace, s);
   const bool filter = set.top_k || with_top_p || with_min_p || (set.top_k_value > 0 && set.top_k_value < V);
