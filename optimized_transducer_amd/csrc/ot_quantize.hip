@@ -12,7 +12,7 @@
 // Bound by memory: every element is read once, 8 per lane in 16-byte loads, and stays in registers
 // between the maximum and the quotient.  Blocks of one row need 16 lanes and four cross-lane steps,
 // and no LDS: 751 992 x 512 bfloat16 takes 239 us, 4.9 TB/s (a large copy reaches 4.7).  A block of
-// 128 x 128 is a workgroup's, 64 elements a lane, one barrier: 5000 x 1000 float32 takes 9.4 us, 2.7
+// 128 x 128 is a workgroup's, 64 elements a lane, one barrier: 5000 x 1000 float32 takes 9.6 us, 2.6
 // TB/s, of which a launch alone is 5.  32 x 512 are a launch, 5.2 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -55,20 +55,18 @@ __device__ __forceinline__ float block_scale(unsigned max_bits) {
   return s < kSmallestScale ? kSmallestScale : s;  // a NaN stays
 }
 
-// Elements [c, c + 8) of row `row`; those at or past D read as 0.  VEC: 16-byte loads (base
-// and row pitch 16-byte aligned, D a multiple of 8, so that 8 elements are all there or none).
-template <class T, bool VEC>
+// Elements [c, c + 8) of row `row`; those at or past D read as 0.  16-byte loads, which a row may
+// start anywhere for (200 000 x 513 float32 113 us, 235 by single elements).  WHOLE: all are there.
+template <class T, bool WHOLE>
 __device__ __forceinline__ void load8(const void *x, int64_t row_stride, int64_t row, int c, int D,
                                       float v[kQuantUnit]) {
   const int64_t at = row * row_stride + c;
-  if (!VEC) {
+  if constexpr (!WHOLE) {
 #pragma unroll
     for (int i = 0; i < kQuantUnit; ++i) v[i] = c + i < D ? load_element<T>(x, at + i) : 0.f;
-  } else if (c >= D) {
-#pragma unroll
-    for (int i = 0; i < kQuantUnit; ++i) v[i] = 0.f;
   } else if constexpr (sizeof(T) == 4) {
-    const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(x) + at);
+    typedef f32x4 unaligned __attribute__((aligned(4)));
+    const unaligned *p = reinterpret_cast<const unaligned *>(static_cast<const float *>(x) + at);
     const f32x4 a = p[0], b = p[1];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -76,7 +74,8 @@ __device__ __forceinline__ void load8(const void *x, int64_t row_stride, int64_t
       v[4 + i] = b[i];
     }
   } else {
-    const u32x4 a = *reinterpret_cast<const u32x4 *>(static_cast<const unsigned short *>(x) + at);
+    typedef u32x4 unaligned __attribute__((aligned(2)));
+    const u32x4 a = *reinterpret_cast<const unaligned *>(static_cast<const unsigned short *>(x) + at);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const unsigned w = a[i];
@@ -87,7 +86,6 @@ __device__ __forceinline__ void load8(const void *x, int64_t row_stride, int64_t
 }
 
 // e4m3(v / scale) to values[row, c .. c + 8)
-template <bool VEC>
 __device__ __forceinline__ void store8(const float v[kQuantUnit], float scale, unsigned char *values,
                                        int64_t row, int c, int D) {
   unsigned w[2];
@@ -97,12 +95,11 @@ __device__ __forceinline__ void store8(const float v[kQuantUnit], float scale, u
     w[h] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2] / scale, v[4 * h + 3] / scale, t, true);
   }
   unsigned char *p = values + row * D + c;
-  if (VEC) {
-    if (c < D) {
-      const u32x2 t = {w[0], w[1]};
-      *reinterpret_cast<u32x2 *>(p) = t;
-    }
-  } else {
+  if (c + kQuantUnit <= D) {
+    typedef u32x2 unaligned __attribute__((aligned(1)));
+    const u32x2 t = {w[0], w[1]};
+    *reinterpret_cast<unaligned *>(p) = t;
+  } else if (c < D) {
 #pragma unroll
     for (int i = 0; i < kQuantUnit; ++i)
       if (c + i < D) p[i] = (unsigned char)(w[i / 4] >> (8 * (i & 3)));
@@ -117,7 +114,7 @@ __device__ __forceinline__ unsigned max8(const float v[kQuantUnit]) {
 }
 
 // blocks of 128 elements of one row: 16 lanes each
-template <class T, bool VEC>
+template <class T>
 __global__ __launch_bounds__(kBlock) void quantize_rows_kernel(const void *__restrict__ x,
                                                                int64_t row_stride, int64_t rows, int D,
                                                                int nblocks,
@@ -130,15 +127,16 @@ __global__ __launch_bounds__(kBlock) void quantize_rows_kernel(const void *__res
     const int64_t row = u / nblocks;
     const int c = (int)(u - row * nblocks) * kQuantBlock + l * kQuantUnit;
     float v[kQuantUnit];
-    load8<T, VEC>(x, row_stride, row, c, D, v);
+    if (c + kQuantUnit <= D) load8<T, true>(x, row_stride, row, c, D, v);
+    else load8<T, false>(x, row_stride, row, c, D, v);
     const float s = block_scale(group16_max(max8(v)));
-    store8<VEC>(v, s, values, row, c, D);
+    store8(v, s, values, row, c, D);
     if (l == 0) scale[u] = s;
   }
 }
 
 // blocks of 128 x 128: one workgroup each, 8 rows per group of 16 lanes
-template <class T, bool VEC>
+template <class T>
 __global__ __launch_bounds__(kBlock) void quantize_tiles_kernel(const void *__restrict__ x,
                                                                 int64_t row_stride, int64_t rows, int D,
                                                                 int nblocks,
@@ -152,13 +150,25 @@ __global__ __launch_bounds__(kBlock) void quantize_tiles_kernel(const void *__re
   const int c = (int)(blockIdx.x - tile_row * nblocks) * kQuantBlock + l * kQuantUnit;
   float v[kRows][kQuantUnit];
   unsigned m = 0;
+  // (one branch around all loads, so that they are on their way together; rows past the end read
+  // the last one)
+  if (c + kQuantUnit <= D) {
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const int64_t row = row0 + i * kQuantGroups;
-    load8<T, VEC>(x, row_stride, min(row, rows - 1), row < rows ? c : D, D, v[i]);
+    for (int i = 0; i < kRows; ++i)
+      load8<T, true>(x, row_stride, min(row0 + i * kQuantGroups, rows - 1), c, D, v[i]);
+  } else if (c < D) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      load8<T, false>(x, row_stride, min(row0 + i * kQuantGroups, rows - 1), c, D, v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int k = 0; k < kQuantUnit; ++k) v[i][k] = 0.f;
   }
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) m = max(m, max8(v[i]));
+  for (int i = 0; i < kRows; ++i)
+    if (row0 + i * kQuantGroups < rows) m = max(m, max8(v[i]));
   m = group16_max(m);
   m = max(m, (unsigned)__shfl_xor((int)m, 16, kWave));
   m = max(m, (unsigned)__shfl_xor((int)m, 32, kWave));
@@ -170,7 +180,7 @@ __global__ __launch_bounds__(kBlock) void quantize_tiles_kernel(const void *__re
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     const int64_t row = row0 + i * kQuantGroups;
-    if (row < rows) store8<VEC>(v[i], s, values, row, c, D);
+    if (row < rows) store8(v[i], s, values, row, c, D);
   }
   if (threadIdx.x == 0) scale[blockIdx.x] = s;
 }
@@ -179,29 +189,17 @@ template <class T>
 static int launch_quantize(const void *x, int64_t row_stride, int64_t rows, int32_t D, int32_t block_rows,
                            unsigned char *values, float *scale, hipStream_t s) {
   const int nblocks = (D + kQuantBlock - 1) / kQuantBlock;
-  const int64_t size = sizeof(T) == 4 ? 4 : 2;
-  const bool vec = D % kQuantUnit == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
-                   (rows == 1 || row_stride * size % 16 == 0) &&
-                   (reinterpret_cast<uintptr_t>(values) & 7) == 0;
   if (block_rows == 1) {
     const int64_t groups = (rows * nblocks + kQuantGroups - 1) / kQuantGroups;
     const dim3 grid((unsigned)(groups < (1 << 20) ? groups : (1 << 20)));
-    if (vec)
-      hipLaunchKernelGGL((quantize_rows_kernel<T, true>), grid, dim3(kBlock), 0, s, x, row_stride, rows, D,
-                         nblocks, values, scale);
-    else
-      hipLaunchKernelGGL((quantize_rows_kernel<T, false>), grid, dim3(kBlock), 0, s, x, row_stride, rows, D,
-                         nblocks, values, scale);
+    hipLaunchKernelGGL((quantize_rows_kernel<T>), grid, dim3(kBlock), 0, s, x, row_stride, rows, D, nblocks, values,
+                       scale);
   } else {
     const int64_t tiles = (rows + kQuantBlock - 1) / kQuantBlock * nblocks;
     if (tiles > (1 << 23)) return OT_E_TOO_LONG;  // a launch holds 2^32 threads at most
     const dim3 grid((unsigned)tiles);
-    if (vec)
-      hipLaunchKernelGGL((quantize_tiles_kernel<T, true>), grid, dim3(kBlock), 0, s, x, row_stride, rows, D,
-                         nblocks, values, scale);
-    else
-      hipLaunchKernelGGL((quantize_tiles_kernel<T, false>), grid, dim3(kBlock), 0, s, x, row_stride, rows, D,
-                         nblocks, values, scale);
+    hipLaunchKernelGGL((quantize_tiles_kernel<T>), grid, dim3(kBlock), 0, s, x, row_stride, rows, D, nblocks, values,
+                       scale);
   }
   return (int)hipGetLastError();
 }
