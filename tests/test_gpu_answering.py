@@ -37,7 +37,8 @@ def _check_quantize(x, block_rows):
 @pytest.mark.parametrize("block_rows", [1, 128])
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("rows,D", [(1, 1), (1, 128), (3, 7), (2, 127), (5, 129), (127, 136), (128, 128), (129, 256),
-                                    (300, 500), (1000, 512), (33, 1000), (2, 4096), (257, 2000)])
+                                    (300, 500), (1000, 512), (33, 1000), (2, 4096), (257, 2000), (200, 513), (131, 1021),
+                                    (3, 4095)])
 def test_quantize(rows, D, dtype, block_rows, device):
     rng = np.random.default_rng(rows * 31 + D)
     x = torch.from_numpy((rng.standard_normal((rows, D)) * np.exp(rng.standard_normal((rows, 1)) * 3)).astype(np.float32))
