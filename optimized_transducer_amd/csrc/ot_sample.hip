@@ -884,12 +884,13 @@ struct Sampler {
   }
 
   // Where the running sum, `run` in front of chunk j, passes the target in it: in the first lane
-  // whose sum does, else the last one with a weight, and there in the first element that does,
-  // else the last one with a weight (sums in another order can fall short of each other's borders
-  // by their rounding).  mine, upto: the lane's sum and the scan over the lanes.
+  // with a weight whose sum does (pass, some), else the last one with a weight, and there in the
+  // first element that does, else the last one with a weight (sums in another order can fall short
+  // of each other's borders by their rounding, and the scan's can grow by one over a lane that adds
+  // nothing).  mine, upto: the lane's sum and the scan over the lanes.
   __device__ __forceinline__ void find(const double t[VEC], const float *y, int i, double run, double mine, double upto,
                                        double target, uint64_t pass, uint64_t some, int &symbol, float &logit) const {
-    const int l = pass ? __builtin_ctzll(pass) : 63 - __builtin_clzll(some);
+    const int l = pass & some ? __builtin_ctzll(pass & some) : 63 - __builtin_clzll(some);
     double c = run + (upto - mine);
     int at = -1;
     bool found = false;
@@ -985,7 +986,7 @@ struct Sampler {
           const uint64_t some = __ballot(mine > 0.0);
           if (some) {
             find(t, y, i, run, mine, upto, target, pass, some, last, last_logit);
-            if (pass) symbol = last;
+            if (pass & some) symbol = last;
           }
           run += chunk;
         });

@@ -1,0 +1,91 @@
+"""sample_symbols where the draw is delicate: entries without a weight beside the border, small
+numbers.
+
+A log-probability is a difference in float32 of an exponent and a logarithm, each rounded."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import optimized_transducer_amd as ot
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+SMALL = 1e-30  # a min_p that takes the kernels with cuts and cuts nothing here
+
+# who works on a row: (V, settings); entries beyond those of a test are -inf
+PATHS = {"batch": (256, {}), "batch, two chunks": (512, {}), "wave": (256, {"min_p": SMALL}),
+         "4 waves": (2000, {}), "8 waves": (8000, {"min_p": SMALL}), "16 waves": (16000, {}),
+         "few": (2000, {"top_k": 512}), "few of a long row": (20000, {"top_k": 512}),
+         "read in every step": (20000, {"min_p": SMALL}), "top_k of a row read in every step": (20000, {"top_k": 600}),
+         "slices": (40000, {}), "slices, min_p": (40000, {"min_p": SMALL})}
+
+
+def _to_device(x, V, dtype, device):
+    """x (rows, n) at the front of rows of V, the rest -inf."""
+    full = torch.full((x.shape[0], V), -math.inf, dtype=DT[dtype], device=device)
+    full[:, :x.shape[1]] = torch.from_numpy(x.astype(np.float32)).to(device).to(DT[dtype])
+    return full
+
+
+def _check_log_prob(got, z, total):
+    """got (float32) of entries at exponent z with weights of `total` remaining."""
+    want = z - np.log(total)
+    tol = 2.0 ** -23 * (np.abs(z) + np.abs(np.log(total)) + np.abs(want))
+    assert (np.abs(got.astype(np.float64) - want) <= tol).all()
+
+
+def _two_halves(rng, rows, vec):
+    """Rows of 64 lanes of `vec` entries, lanes 32-63 the entries of lanes 0-31 again: half of the
+    weights lies in front of lane 32.  From a random lane on the end of each half is empty."""
+    half = rng.standard_normal((rows, 32, vec)) * 2
+    half[np.arange(32)[None, :] >= rng.integers(20, 32, rows)[:, None]] = -np.inf
+    return np.concatenate([half, half], 1).reshape(rows, 64 * vec)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("path", list(PATHS))
+def test_the_draw_never_leaves_what_remains(path, dtype, device):
+    """u = 1/2 falls on the border between two halves of equal weights with masked entries around it:
+    the answer is one of the two entries at the border, never a masked one."""
+    V, settings = PATHS[path]
+    rows, vec = 4000 if V <= 2000 else 1000, 4 if dtype == "f32" else 8
+    V = max(V, 64 * vec)
+    x = _two_halves(np.random.default_rng(V), rows, vec)
+    t = _to_device(x, V, dtype, device)
+    x = t[:, :64 * vec].double().cpu().numpy()
+    symbols, log_probs = ot.sample_symbols(t, torch.full((rows,), 0.5, device=device), **settings)
+    s, lp = symbols.cpu().numpy(), log_probs.cpu().numpy()
+    n = 32 * vec
+    last = n - 1 - np.argmax(np.isfinite(x[:, :n])[:, ::-1], 1)
+    first = n + np.argmax(np.isfinite(x[:, n:]), 1)
+    at = np.arange(rows)
+    assert (np.isfinite(x[at, np.clip(s, 0, 64 * vec - 1)]) & (s >= 0) & (s < 64 * vec)).all()
+    assert ((s == last) | (s == first)).all()
+    m = x.max(1)
+    _check_log_prob(lp, x[at, s] - m, np.exp(x - m[:, None]).sum(1))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [256, 2000, 20000])
+def test_the_draw_never_takes_what_min_p_has_cut(V, dtype, device):
+    """The same with entries that min_p leaves out in place of masked ones, with and without top_k."""
+    vec = 4 if dtype == "f32" else 8
+    V = max(V, 64 * vec)
+    rows = 4000 if V <= 2000 else 500
+    x = _two_halves(np.random.default_rng(V + 1), rows, vec)
+    x[np.isneginf(x)] = -60.0
+    t = _to_device(x, V, dtype, device)
+    x = t[:, :64 * vec].double().cpu().numpy()
+    u = torch.full((rows,), 0.5, device=device)
+    n = 32 * vec
+    last = n - 1 - np.argmax((x > -50)[:, :n][:, ::-1], 1)
+    first = n + np.argmax((x > -50)[:, n:], 1)
+    for settings in ({}, {"top_k": 64 * vec}):
+        s, lp = (a.cpu().numpy() for a in ot.sample_symbols(t, u, min_p=1e-12, **settings))
+        assert ((s == last) | (s == first)).all()
+        m = x.max(1)
+        w = np.where(x > -50, np.exp(x - m[:, None]), 0.0)
+        _check_log_prob(lp, x[np.arange(rows), s] - m, w.sum(1))

@@ -1,0 +1,52 @@
+"""The order of additions of a draw, without a GPU: where sums over lanes do not grow, and that a draw
+does not leave the entries with a weight there."""
+import numpy as np
+import pytest
+
+import answering_oracle as ao
+import draw_model
+
+
+def two_halves(rng, rows, vec):
+    """Rows of 64 lanes of `vec` entries, lanes 32-63 the entries of lanes 0-31 again: half of the
+    weights lies in front of lane 32.  From a random lane on the end of each half is empty."""
+    half = rng.standard_normal((rows, 32, vec)) * 2
+    half[np.arange(32)[None, :] >= rng.integers(20, 32, rows)[:, None]] = -np.inf
+    return np.concatenate([half, half], 1).reshape(rows, 64 * vec).astype(np.float32)
+
+
+@pytest.mark.parametrize("vec", [4, 8])
+def test_scan_sums_the_lanes_in_front(vec):
+    v = np.random.default_rng(0).integers(0, 1000, (50, 64)).astype(np.float64)
+    assert np.array_equal(draw_model.scan(v), np.cumsum(v, 1))
+    w = np.random.default_rng(1).integers(0, 9, (50, 64, vec)).astype(np.float64)
+    assert np.array_equal(draw_model.pairwise(w), w.sum(2))
+
+
+@pytest.mark.parametrize("vec", [4, 8])
+def test_draw_stays_among_the_entries_with_a_weight(vec):
+    """Targets between the sums of a lane with the last weight of a half and of an empty lane behind
+    it: such rows are there, and each draws one of the two entries at the border."""
+    rows, n = 3000, 32 * vec
+    x = two_halves(np.random.default_rng(vec), rows, vec)
+    w = draw_model.weights(x.astype(np.float64))
+    upto = draw_model.scan(draw_model.pairwise(w))
+    empty = w.sum(2) == 0
+    target = 0.5 * upto[:, -1:]
+    # the first lane whose sum passes the target is an empty one
+    first = np.argmax(upto > target, 1)
+    assert empty[np.arange(rows), first].sum() > 10
+    got = draw_model.draw(w, np.full(rows, 0.5))
+    front = n - 1 - np.argmax(np.isfinite(x[:, :n])[:, ::-1], 1)
+    behind = n + np.argmax(np.isfinite(x[:, n:]), 1)
+    assert ((got == front) | (got == behind)).all()
+
+
+@pytest.mark.parametrize("vec", [4, 8])
+def test_draw_is_the_oracles_away_from_borders(vec):
+    rng = np.random.default_rng(10 + vec)
+    x = (rng.standard_normal((300, 64 * vec)) * 3).astype(np.float32)
+    x[rng.random(x.shape) < 0.3] = -np.inf
+    u = rng.random(300, dtype=np.float32)
+    got = draw_model.draw(draw_model.weights(x.astype(np.float64)), u.astype(np.float64))
+    assert np.array_equal(got, ao.sample(x, u, 1.0, 0, 1.0, 0.0)[0])
