@@ -1706,7 +1706,8 @@ __global__ __launch_bounds__(kSliceThreads, 2) void slice_draw_kernel(SlicedRows
   const double run = wave_scan(mine.kept), total = lane_value(run, kWave - 1);
   const uint64_t some = __ballot(mine.kept > 0.0), pass = __ballot(mine.kept > 0.0 && run > fmax(u, 0.0) * total);
   const int slice = pass ? __builtin_ctzll(pass) : 63 - __builtin_clzll(some);
-  const double before = slice > 0 ? lane_value(run, slice - 1) : 0.0;
+  // (the scan's sum can grow by a rounding over slices that add nothing, past the target)
+  const double before = slice > 0 ? fmin(lane_value(run, slice - 1), fmax(u, 0.0) * total) : 0.0;
   P p(a, r, slice, lane, wave);
   if (st.cuts) {
 #pragma unroll

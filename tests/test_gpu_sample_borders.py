@@ -89,3 +89,29 @@ def test_the_draw_never_takes_what_min_p_has_cut(V, dtype, device):
         m = x.max(1)
         w = np.where(x > -50, np.exp(x - m[:, None]), 0.0)
         _check_log_prob(lp, x[np.arange(rows), s] - m, w.sum(1))
+
+
+@pytest.mark.parametrize("settings", [{}, {"min_p": SMALL}], ids=["no cuts", "min_p"])
+def test_the_border_between_slices(settings, device):
+    """Slices of 8192 entries, the second 32 of a row as the first, the end of each half empty, and
+    u = 1/2: the last entry in front of the border or the first behind it, not any other of its slice."""
+    rng = np.random.default_rng(64)
+    rows, V = 100, 64 * 8192
+    at = np.sort(rng.choice(8192, (32, 5), replace=False), 1)
+    half = rng.standard_normal((rows, 32, 5)).astype(np.float32) * 2
+    half[np.arange(32)[None, :] >= rng.integers(12, 32, rows)[:, None]] = -np.inf
+    t = torch.full((rows, 64, 8192), -math.inf, device=device)
+    where = torch.from_numpy(at).to(device).expand(rows, 32, 5)
+    h = torch.from_numpy(half).to(device)
+    t[:, :32].scatter_(2, where, h)
+    t[:, 32:].scatter_(2, where, h)
+    symbols, log_probs = ot.sample_symbols(t.view(rows, V), torch.full((rows,), 0.5, device=device), **settings)
+    s = symbols.cpu().numpy()
+    end = np.isfinite(half[:, :, 0]).sum(1) - 1  # the last slice of a half
+    last = end * 8192 + at[end, 4]
+    first = 32 * 8192 + at[0, 0]
+    assert ((s == last) | (s == first)).all(), s[(s != last) & (s != first)][:5]
+    m = half.reshape(rows, -1).max(1).astype(np.float64)
+    x = np.where(s == last, half[np.arange(rows), end, 4], half[:, 0, 0])
+    _check_log_prob(log_probs.cpu().numpy(), x - m,
+                    2 * np.exp(half.reshape(rows, -1).astype(np.float64) - m[:, None]).sum(1))
