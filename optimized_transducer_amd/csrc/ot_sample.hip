@@ -887,11 +887,12 @@ struct Sampler {
   // with a weight whose sum does (pass, some), else the last one with a weight, and there in the
   // first element that does, else the last one with a weight (sums in another order can fall short
   // of each other's borders by their rounding, and the scan's can grow by one over a lane that adds
-  // nothing).  mine, upto: the lane's sum and the scan over the lanes.
-  __device__ __forceinline__ void find(const double t[VEC], const float *y, int i, double run, double mine, double upto,
+  // nothing).  upto: the scan over the lanes.  What lies in front of the lane is the scan's sum at
+  // the lane before, and not the difference of two sums, which loses small weights before a large one.
+  __device__ __forceinline__ void find(const double t[VEC], const float *y, int i, double run, double upto,
                                        double target, uint64_t pass, uint64_t some, int &symbol, float &logit) const {
     const int l = pass & some ? __builtin_ctzll(pass & some) : 63 - __builtin_clzll(some);
-    double c = run + (upto - mine);
+    double c = l > 0 ? run + lane_value(upto, l - 1) : run;
     int at = -1;
     bool found = false;
 #pragma unroll
@@ -930,7 +931,7 @@ struct Sampler {
     for (int j = CHUNKS - 1; j >= 0; --j) {
       const uint64_t some = __ballot(mine[j] > 0.0);
       if (past ? symbol < 0 && some != 0 : before[j] <= target && target < before[j + 1])
-        find(w[j], x[j], first_index(j), before[j], mine[j], upto[j], target,
+        find(w[j], x[j], first_index(j), before[j], upto[j], target,
              __ballot(before[j] + upto[j] > target), some, symbol, logit);
     }
   }
@@ -985,7 +986,7 @@ struct Sampler {
           const uint64_t pass = __ballot(run + upto > target);
           const uint64_t some = __ballot(mine > 0.0);
           if (some) {
-            find(t, y, i, run, mine, upto, target, pass, some, last, last_logit);
+            find(t, y, i, run, upto, target, pass, some, last, last_logit);
             if (pass & some) symbol = last;
           }
           run += chunk;

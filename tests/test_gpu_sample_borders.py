@@ -115,3 +115,33 @@ def test_the_border_between_slices(settings, device):
     x = np.where(s == last, half[np.arange(rows), end, 4], half[:, 0, 0])
     _check_log_prob(log_probs.cpu().numpy(), x - m,
                     2 * np.exp(half.reshape(rows, -1).astype(np.float64) - m[:, None]).sum(1))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("path", list(PATHS))
+def test_small_numbers_find_small_entries_before_a_large_one(path, dtype, device):
+    """Entries of weights around 1e-17 in front of one of weight 1, in the same 16 bytes and before
+    them: numbers in the middle of each one's share draw it."""
+    V, settings = PATHS[path]
+    vec = 4 if dtype == "f32" else 8
+    V = max(V, 64 * vec)
+    x, u, want = [], [], []
+    for base in (0, vec, 5 * vec, 17 * vec, 63 * vec, V // (2 * vec) * vec, (V // vec - 1) * vec):
+        for places in ((0, 1, 2), (0, 1, vec - 1), (1, vec - 2, vec - 1)):
+            row = np.full(V, -np.inf)
+            row[base + np.array(places)] = (-38.5, -40.0, 0.0)
+            if base > 0:
+                row[base - 1], row[base // 2] = -39.0, -40.5
+            at = np.nonzero(np.isfinite(row))[0]
+            run = np.cumsum(np.exp(row[at]))
+            for k in range(len(at)):
+                number = np.float32(((run[k - 1] if k else 0.0) + run[k]) / 2 / run[-1])
+                x.append(row)
+                u.append(number)
+                want.append(at[k])
+    t = _to_device(np.stack(x), V, dtype, device)
+    s, lp = ot.sample_symbols(t, torch.from_numpy(np.array(u, np.float32)).to(device), **settings)
+    got, want = s.cpu().numpy(), np.array(want)
+    assert np.array_equal(got, want), [(i, got[i], want[i]) for i in np.nonzero(got != want)[0][:5]]
+    x = np.stack(x)
+    _check_log_prob(lp.cpu().numpy(), x[np.arange(len(x)), want], np.exp(x).sum(1))

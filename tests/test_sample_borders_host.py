@@ -50,3 +50,20 @@ def test_draw_is_the_oracles_away_from_borders(vec):
     u = rng.random(300, dtype=np.float32)
     got = draw_model.draw(draw_model.weights(x.astype(np.float64)), u.astype(np.float64))
     assert np.array_equal(got, ao.sample(x, u, 1.0, 0, 1.0, 0.0)[0])
+
+
+@pytest.mark.parametrize("vec", [4, 8])
+def test_draw_of_small_numbers(vec):
+    """Entries of small weights in front of a large one in the same lane: their running sums are kept,
+    which the difference of the lane's sum and its own would not."""
+    for lane in (0, 1, 17, 63):
+        x = np.full((1, 64 * vec), -np.inf)
+        x[0, lane * vec + np.arange(3)] = (-38.5, -40.0, 0.0)
+        if lane:
+            x[0, 1] = -39.0
+        w = draw_model.weights(x)
+        at = np.nonzero(np.isfinite(x[0]))[0]
+        run = np.cumsum(w.reshape(-1)[at])
+        middle = (run + np.concatenate([[0.0], run[:-1]])) / 2 / run[-1]
+        got = draw_model.draw(np.repeat(w, len(at), 0), middle)
+        assert np.array_equal(got, at)
