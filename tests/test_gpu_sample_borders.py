@@ -145,3 +145,27 @@ def test_small_numbers_find_small_entries_before_a_large_one(path, dtype, device
     assert np.array_equal(got, want), [(i, got[i], want[i]) for i in np.nonzero(got != want)[0][:5]]
     x = np.stack(x)
     _check_log_prob(lp.cpu().numpy(), x[np.arange(len(x)), want], np.exp(x).sum(1))
+
+
+# (x, T, u): a row (x, 0) at temperature T, where u is less than 5e-15 of it below the first entry's
+# share 1 / (1 + exp(-x / T)), which 64 bits tell apart by ten roundings or more
+CLOSE = [("-0x1.a8fdb2p+1", 1.375, "0x1.501af8p-4"), ("-0x1.feaf5ep+0", 0.640625, "0x1.5c74d2p-5"),
+         ("-0x1.feaf5ep+1", 1.28125, "0x1.5c74d2p-5"), ("-0x1.acbf0ap-1", 2.421875, "0x1.a85b28p-2"),
+         ("-0x1.a8fdb2p+0", 0.6875, "0x1.501af8p-4"), ("-0x1.b44cb4p+1", 0.578125, "0x1.67893ap-9")]
+
+
+@pytest.mark.parametrize("path", list(PATHS))
+def test_weights_are_those_of_64_bits(path, device):
+    """Numbers a few roundings of 64 bits away from the border between two entries."""
+    V, settings = PATHS[path]
+    x = np.full((len(CLOSE), V), -np.inf, np.float32)
+    for i, (v, _, _) in enumerate(CLOSE):
+        x[i, 17 * i] = float.fromhex(v)
+        x[i, V // 2 + i] = 0.0
+    T = torch.tensor([t for _, t, _ in CLOSE], device=device)
+    u = torch.tensor([float.fromhex(n) for _, _, n in CLOSE], device=device)
+    s, _ = ot.sample_symbols(_to_device(x, V, "f32", device), u, temperature=T, **settings)
+    assert s.tolist() == [17 * i for i in range(len(CLOSE))]
+    above = torch.nextafter(u, torch.ones_like(u))
+    s, _ = ot.sample_symbols(_to_device(x, V, "f32", device), above, temperature=T, **settings)
+    assert s.tolist() == [V // 2 + i for i in range(len(CLOSE))]
