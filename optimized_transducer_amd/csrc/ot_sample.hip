@@ -291,10 +291,11 @@ __device__ __forceinline__ void load_logits(const void *row, int i, int V, float
 // ln(2)^k / k! for k = 13 down to 1: read once into scalar registers, where literals would be moved
 // into vector registers in front of every use
 constexpr int kExpTerms = 13;
-__constant__ double kExpSeries[kExpTerms] = {1.3691488853904128e-12, 2.5678435993488206e-11, 4.4455382718708115e-10, 7.0549116208011233e-09, 1.0178086009239699e-07,
-                                      1.3215486790144307e-06, 1.5252733804059841e-05, 1.5403530393381609e-04,
-                                      1.3333558146428443e-03, 9.6181291076284772e-03, 5.5504108664821580e-02,
-                                      2.4022650695910072e-01, 6.9314718055994531e-01};
+__constant__ double kExpSeries[kExpTerms] = {
+    1.3691488853904128e-12, 2.5678435993488206e-11, 4.4455382718708116e-10, 7.0549116208011234e-09,
+    1.0178086009239700e-07, 1.3215486790144310e-06, 1.5252733804059841e-05, 1.5403530393381609e-04,
+    1.3333558146428443e-03, 9.6181291076284769e-03, 5.5504108664821583e-02, 2.4022650695910072e-01,
+    6.9314718055994529e-01};
 
 // exp((x - m) / T) = 2^n * 2^f with n the nearest integer to (x - m) * c, c = log2(e) / T, and
 // 2^f the exponential series of f * ln 2, |f| <= 1/2, up to the 13th power: within 1.4e-16 = 2^-52.7 of
