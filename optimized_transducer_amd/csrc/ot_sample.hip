@@ -327,12 +327,10 @@ struct Drawn {
   float log_prob;
 };
 
-// (x - m) / T - log(total); the largest entry always remains, so total = 1 + the others' sum
+// (x - m) / T - log(total) in 64 bits, rounded once: one per row (with the parts in float32, each
+// rounded, it is up to 1.7 times as far off)
 __device__ __forceinline__ float log_probability(float logit, float m, float T, double total) {
-  const float rest = (float)(total - 1.0), t = 1.0f + rest;
-  const float small = logf(t) + (rest - (t - 1.0f)) / t;
-  const float z = m - logit > 3e38f || T < 1e-30f || T > 1e30f ? (float)(((double)logit - m) / T) : (logit - m) / T;
-  return z - (rest < 1.0f ? small : logf((float)total));
+  return (float)(((double)logit - m) / T - log(total));
 }
 
 // Draws from a row with a finite largest entry m at a temperature above 0.  Every thread of the

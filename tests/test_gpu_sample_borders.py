@@ -1,13 +1,17 @@
 """sample_symbols where the draw is delicate: entries without a weight beside the border, small
-numbers.
+numbers, weights and log-probabilities to the last bit that is promised.
 
-A log-probability is a difference in float32 of an exponent and a logarithm, each rounded."""
+A log-probability is log(w / total) in 64 bits, rounded once to float32.  Its 64-bit error: weights
+are exp of (x - m) / T with three roundings of the exponent and a few of the series, which move the
+total by at most 3 (log V + 1) 2^-53 of it, the sums add at most 60 roundings, the difference and the
+logarithm three, and an exponent of z three of |z|: below 2^-46 (1 + |z|) in all."""
 import math
 
 import numpy as np
 import pytest
 import torch
 
+import answering_oracle as ao
 import optimized_transducer_amd as ot
 
 pytestmark = pytest.mark.gpu
@@ -33,7 +37,7 @@ def _to_device(x, V, dtype, device):
 def _check_log_prob(got, z, total):
     """got (float32) of entries at exponent z with weights of `total` remaining."""
     want = z - np.log(total)
-    tol = 2.0 ** -23 * (np.abs(z) + np.abs(np.log(total)) + np.abs(want))
+    tol = 2.0 ** -24 * np.abs(want) + 2.0 ** -46 * (1 + np.abs(z))
     assert (np.abs(got.astype(np.float64) - want) <= tol).all()
 
 
@@ -169,3 +173,35 @@ def test_weights_are_those_of_64_bits(path, device):
     above = torch.nextafter(u, torch.ones_like(u))
     s, _ = ot.sample_symbols(_to_device(x, V, "f32", device), above, temperature=T, **settings)
     assert s.tolist() == [V // 2 + i for i in range(len(CLOSE))]
+
+
+@pytest.mark.parametrize("V,settings", [(50, {}), (500, {}), (500, {"min_p": 0.01}), (1000, {"top_p": 0.9}),
+                                        (3001, {}), (5000, {"top_k": 200, "top_p": 0.95}), (15000, {"top_p": 0.8}),
+                                        (30000, {"top_k": 700}), (50000, {}), (50000, {"top_p": 0.9, "min_p": 1e-4})])
+@pytest.mark.parametrize("temperature", [1.0, 0.3, 7.0])
+def test_log_probs_are_rounded_once(V, settings, temperature, device):
+    """The logarithm of 64 bits, rounded to float32: rows from flat to one entry of nearly all."""
+    rng = np.random.default_rng(V)
+    rows = 600 if V <= 5000 else 60
+    x = (rng.standard_normal((rows, V)) * rng.choice([0.1, 1, 3, 10], (rows, 1))).astype(np.float32)
+    x[:, 0] += rng.choice([0.0, 5.0, 15.0, 25.0], rows).astype(np.float32)
+    u = rng.random(rows).astype(np.float32)
+    s, lp = ot.sample_symbols(torch.from_numpy(x).to(device), torch.from_numpy(u).to(device),
+                              temperature=temperature, **settings)
+    s, lp = s.cpu().numpy(), lp.cpu().numpy()
+    top_k, top_p, min_p = settings.get("top_k", 0), settings.get("top_p", 1.0), settings.get("min_p", 0.0)
+    T = np.float64(np.float32(temperature))
+    z, total = np.zeros(rows), np.zeros(rows)
+    for r in range(rows):
+        want, _ = ao.sample_row(x[r], float(u[r]), temperature, top_k, top_p, min_p)
+        assert want == s[r]
+        row = (x[r].astype(np.float64) - x[r].max()) / T
+        w = np.sort(np.exp(row))[::-1]
+        if top_k:
+            w = w[:top_k]
+        if top_p < 1:
+            run = np.cumsum(w)
+            w = w[:max(1, int((np.concatenate([[0.0], run[:-1]]) < np.float64(np.float32(top_p)) * run[-1]).sum()))]
+        total[r] = math.fsum(w[w >= np.float64(np.float32(min_p))])
+        z[r] = row[s[r]]
+    _check_log_prob(lp, z, total)
