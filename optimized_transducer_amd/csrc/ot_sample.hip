@@ -14,7 +14,7 @@
 //
 // Which index a symbol falls on, or where top_p cuts, hangs on the last bits of a sum: weights
 // and sums are 64-bit.  This chip's vector units do 64-bit multiply-adds at the rate of
-// (unpacked) 32-bit ones, so a weight costs 21 such instructions (a range reduction and a
+// (unpacked) 32-bit ones, so a weight costs 19 such instructions (a range reduction and a
 // polynomial for 2^f) where a 32-bit one through the hardware's 2^x costs 8 and the transcendental
 // unit.
 //
@@ -288,30 +288,35 @@ __device__ __forceinline__ void load_logits(const void *row, int i, int V, float
   }
 }
 
-// ln(2)^k / k! for k = 13 down to 1: read once into scalar registers, where literals would be moved
-// into vector registers in front of every use
-constexpr int kExpTerms = 13;
+// Coefficients of f^11 down to f in 2^f = 1 + f * q(f): q interpolates (2^f - 1) / f at the 11 Chebyshev
+// nodes of [-1/2, 1/2].  Read once into scalar registers, where literals would be moved into vector
+// registers in front of every use.
+constexpr int kExpTerms = 11;
 __constant__ double kExpSeries[kExpTerms] = {
-    1.3691488853904128e-12, 2.5678435993488206e-11, 4.4455382718708116e-10, 7.0549116208011234e-09,
-    1.0178086009239700e-07, 1.3215486790144310e-06, 1.5252733804059841e-05, 1.5403530393381609e-04,
-    1.3333558146428443e-03, 9.6181291076284769e-03, 5.5504108664821583e-02, 2.4022650695910072e-01,
-    6.9314718055994529e-01};
+    4.4549605981865186e-10, 7.0725859492692234e-09, 1.0178062445845774e-07, 1.3215442587921689e-06,
+    1.5252733829836119e-05, 1.5403530441736050e-04, 1.3333558146416936e-03, 9.6181291076068882e-03,
+    5.5504108664821597e-02, 2.4022650695910097e-01, 6.9314718055994529e-01};
 
-// exp((x - m) / T) = 2^n * 2^f with n the nearest integer to (x - m) * c, c = log2(e) / T, and
-// 2^f the exponential series of f * ln 2, |f| <= 1/2, up to the 13th power: within 1.4e-16 = 2^-52.7 of
-// 2^f over 4e7 values of f (the 11th power leaves 8.7e-15).  The exponent has three roundings, so a
-// weight is within (|(x - m) / T| + 1) * 2^-51.  Exactly 1 at x = m, exactly 0 at x = -inf.
+// 2^t, t >= -1100, as 2^n * 2^f with n the nearest integer to t and 2^f the polynomial above for
+// |f| <= 1/2: within 1.4e-16 = 2^-52.7 of it over 4e7 values of f (the exponential series needs the
+// 13th power for that: 751 992 x 500 float32 524 us and 502 so)
+__device__ __forceinline__ double power_of_2(double t) {
+  const double n = __builtin_rint(t), f = t - n;
+  double p = kExpSeries[0];
+#pragma unroll
+  for (int k = 1; k < kExpTerms; ++k) p = __builtin_fma(p, f, kExpSeries[k]);
+  p = __builtin_fma(p, f, 1.0);
+  return __builtin_ldexp(p, (int)n);
+}
+
+// exp((x - m) / T) = 2^((x - m) * c), c = log2(e) / T.  The exponent has three roundings, so a weight is
+// within (|(x - m) / T| + 1) * 2^-51.  Exactly 1 at x = m, exactly 0 at x = -inf.
 struct Weight {
   double m, c;
   __device__ __forceinline__ Weight(float m_, float T) : m(m_), c(1.4426950408889634074 / (double)T) {}
   __device__ __forceinline__ double operator()(float x) const {
     // (T = inf and x = -inf make a NaN of the product, which fmax drops)
-    const double t = __builtin_fmax(((double)x - m) * c, -1100.0), n = __builtin_rint(t), f = t - n;
-    double p = kExpSeries[0];
-#pragma unroll
-    for (int k = 1; k < kExpTerms; ++k) p = __builtin_fma(p, f, kExpSeries[k]);
-    p = __builtin_fma(p, f, 1.0);
-    return __builtin_ldexp(p, (int)n);
+    return power_of_2(__builtin_fmax(((double)x - m) * c, -1100.0));
   }
 };
 
@@ -327,10 +332,14 @@ struct Drawn {
   float log_prob;
 };
 
-// (x - m) / T - log(total) in 64 bits, rounded once: one per row (with the parts in float32, each
-// rounded, it is up to 1.7 times as far off)
+// (x - m) / T - log(total) in 64 bits, rounded once; total >= 1.  log(total) = a + 2 artanh((total - e) /
+// (total + e)) with a = log of e = 2^b, b the hardware's logarithm of 32 bits: artanh's first term is
+// enough (its argument is below 2^-20, the next term below 2^-60), and the polynomial of the weights
+// serves again (the library's logarithm keeps 12 more registers of constants over a kernel's loop:
+// 751 992 x 500 float32 519 us and 504 so, 4096 x 16 000 with top_p 712 and 629)
 __device__ __forceinline__ float log_probability(float logit, float m, float T, double total) {
-  return (float)(((double)logit - m) / T - log(total));
+  const double b = __builtin_amdgcn_logf((float)total), e = power_of_2(b);
+  return (float)(((double)logit - m) / T - (b * 0.69314718055994531 + 2.0 * ((total - e) / (total + e))));
 }
 
 // Draws from a row with a finite largest entry m at a temperature above 0.  Every thread of the
