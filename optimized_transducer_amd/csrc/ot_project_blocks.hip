@@ -35,6 +35,8 @@ constexpr int kSmallCols = 64;     // vocabulary entries of a workgroup of the s
 constexpr int kWideCols = 64, kWideTiles = 2, kWideRows = kWavesPerBlock * kWideTiles * 16;
 constexpr int kPartCols = 64;      // least vocabulary entries behind one partial log-sum-exp
 
+constexpr float kLargest = 3.402823466385288598e38f;  // the largest finite float32
+
 // a running log-sum-exp as (largest value, sum of exp(value - largest))
 struct LogSum {
   float m, s;
@@ -352,14 +354,15 @@ struct WideProject {
     }
     if constexpr (DEN) {
       // running log-sum-exp of this lane's share of its rows, relative to ref, which follows the
-      // largest value so far at a distance of at most 20
+      // largest value so far at a distance of at most 20; it starts at the lowest finite value, so that
+      // rows of no larger logits keep their sum, and stays finite, so that differences do
       constexpr float kLog2e = 1.44269502162933349609375f;
 #pragma unroll
       for (int t = 0; t < kWideTiles; ++t) {
         float top = acc[0][t][0];
 #pragma unroll
         for (int i = 1; i < kGroup; ++i) top = fmaxf(top, acc[i / 4][t][i % 4]);
-        const float to = top > ref[t] + 20.f ? fminf(top, 3e38f) : ref[t];
+        const float to = top > ref[t] + 20.f ? fminf(top, kLargest) : ref[t];
         float s = sum[t] * __builtin_amdgcn_exp2f((ref[t] - to) * kLog2e);
         // (a difference first: in powers of 2 the rounding of a large `to` would be an exponent)
 #pragma unroll
@@ -435,7 +438,7 @@ __global__ __launch_bounds__(kBlock, 2) void project_blocks_wide_kernel(
         p.x[t][b][2 * q + 1] = widen(c[2], c[3]);
       }
     }
-    p.ref[t] = -1e30f;
+    p.ref[t] = -kLargest;
     p.sum[t] = 0.f;
   }
   p.xs = s_xs[p.wave];
@@ -585,7 +588,7 @@ __global__ __launch_bounds__(kBlock, COLS == 64 ? 3 : 2) void project_blocks_dee
     const int64_t row = min(row0 + 16 * t + r, rows - 1);
     p.x[t] = x + row * D;
     p.xs[t] = xs + row * p.nblocks;
-    p.e.ref[t] = -1e30f;
+    p.e.ref[t] = -kLargest;
     p.e.sum[t] = 0.f;
   }
   p.load(0, s_w0);
