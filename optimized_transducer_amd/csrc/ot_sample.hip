@@ -326,6 +326,10 @@ __device__ __forceinline__ unsigned order_key(float x) {
   return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
+__device__ __forceinline__ float key_value(unsigned key) {
+  return __builtin_bit_cast(float, key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
+}
+
 // one row's answer
 struct Drawn {
   int symbol;
@@ -779,6 +783,7 @@ struct Sampler {
     return ok;
   }
 
+  static constexpr int kNearSteps = 4;
   __device__ __forceinline__ void keep_top_p(float p, float lowest) {
     double total;
     int none;
@@ -797,15 +802,27 @@ struct Sampler {
     if (V <= kSampleBins * kSampleBins && cut_in_one_bin(want, from)) return;
     double rough, sum;
     float v = select<true>(want, from, rough);
+    // Where the entries above v reach `want` already, or those at it do not, v is somewhere else: next
+    // to it for a few steps, and then by halving what is left of the values' keys (32-bit sums of many
+    // weights in one bin can be off by thousands of entries, and stop growing at 2^24 times a weight).
+    unsigned below = order_key(lowest) - 1, beyond = order_key(m) + 1;  // v's key is between them
     int at_v, went = 0;
     double wv;
-    for (;;) {
+    bool last = false;
+    for (int step = 0;; ++step) {
       sum_above<false>(v, sum, at_v);
       wv = weight(v);
-      // where the entries above v reach `want` already, or those at it do not: the next value
       const int go = sum >= want && v < m ? 1 : sum + at_v * wv < want && v > lowest ? -1 : 0;
-      if (go == 0 || go == -went) break;  // (back and forth: the border lies within a rounding)
-      went = go;
+      if (last || go == 0 || go == -went) break;  // (back and forth: the border lies within a rounding)
+      if (go > 0) below = order_key(v);
+      else beyond = order_key(v);
+      went = step < kNearSteps ? go : 0;
+      last = step >= kNearSteps && beyond - below <= 1;  // nothing left: a rounding again
+      if (step >= kNearSteps && !last) {
+        v = key_value(below + (beyond - below) / 2);  // (`go` is not 0 where no entry is)
+        continue;
+      }
+      if (last) v = key_value(below);
       float up = kInf, down = OT_NEG_INF;
       each([&](int, int, const float *y) {
 #pragma unroll
@@ -815,7 +832,7 @@ struct Sampler {
         }
       });
       g.extremes(down, up);
-      v = go > 0 ? up : down;
+      v = last || go > 0 ? up : down;
     }
     // of the entries at v, number j (from 0) remains if sum + j * wv < want
     int n = at_v;

@@ -205,3 +205,43 @@ def test_log_probs_are_rounded_once(V, settings, temperature, device):
         total[r] = math.fsum(w[w >= np.float64(np.float32(min_p))])
         z[r] = row[s[r]]
     _check_log_prob(lp, z, total)
+
+
+def _near(rng, V):
+    """An entry of weight 1, the others within 2e-6 of weight 0.52: sums of 32 bits round every one of
+    them the same way."""
+    x = (math.log(0.52) + 1e-6 * rng.random(V)).astype(np.float32)
+    x[V // 3] = 0.0
+    return x, 1.0
+
+
+def _clusters(rng, V):
+    """Two thirds of the weights, nearly equal ones, in one bin of 256 between the largest entry and
+    the smallest, and a third in another: more of them than 32-bit sums count."""
+    x = rng.random(V, dtype=np.float32)
+    x[rng.random(V) < 1 / 3] -= np.float32(10.0)
+    x[V // 5] = 1000.0
+    return x, 1e6
+
+
+@pytest.mark.parametrize("make,V,top_p", [(_near, 700001, 0.5), (_near, 700001, 0.9), (_clusters, 700001, 0.6),
+                                          (_clusters, 30000001, 0.6), (_clusters, 30000001, 0.9)])
+def test_top_p_where_sums_of_32_bits_are_far_off(make, V, top_p, device):
+    """Rows of a workgroup each, of many near weights: the cut is found in a bounded number of passes."""
+    x, T = make(np.random.default_rng(V), V)
+    u = np.array([0.3, 0.999], np.float32)
+    t = torch.from_numpy(x).to(device)
+    s, lp = ot.sample_symbols(t.expand(2, V), torch.from_numpy(u).to(device), temperature=T, top_p=top_p)
+    z = (x.astype(np.float64) - x.max()) / T
+    w = np.exp(z)
+    order = np.sort(x)[::-1]
+    run = np.cumsum(np.exp((order.astype(np.float64) - x.max()) / T))
+    n = int(np.searchsorted(run, np.float64(np.float32(top_p)) * run[-1])) + 1  # entries that remain
+    kept = x > order[n - 1]
+    at = np.nonzero(x == order[n - 1])[0]
+    kept[at[:n - int(kept.sum())]] = True
+    run = np.cumsum(np.where(kept, w, 0.0))
+    want = [int(np.searchsorted(run, float(v) * run[-1], side="right")) for v in u]
+    assert s.tolist() == want
+    want_lp = z[want] - math.log(run[-1])
+    assert (np.abs(lp.double().cpu().numpy() - want_lp) <= 2.0 ** -24 * np.abs(want_lp) + 2.0 ** -30).all()
