@@ -62,7 +62,7 @@ def project_joiner_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Ten
       ``denominators`` (rows,) float32 = the log-sum-exp of the float32 logits (before the
       rounding to ``logits_dtype``), for ``transducer_loss(..., denominators=...)``, or None.
     """
-    _no_gradient("project_joiner_fp8", x_scale, weight_scale, bias)
+    _no_gradient("project_joiner_fp8", x, x_scale, weight, weight_scale, bias)
     return _optimized_transducer.joiner_project_blocks(x, x_scale, weight, weight_scale, bias,
                                                        logits_dtype, denominators)
 

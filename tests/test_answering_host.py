@@ -136,3 +136,14 @@ def test_c_abi_refuses_bad_arguments():
     for bad in (dict(logits=odd), dict(logits=ctypes.c_void_p(66)), dict(uniform=odd), dict(t=odd), dict(k=odd),
                 dict(p=odd), dict(m=odd), dict(symbols=odd), dict(log_probs=odd)):
         assert sample(**bad) == -3, bad
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_projection_refuses_every_operand_that_asks_for_a_gradient(which):
+    f8 = lambda *shape: torch.zeros(shape, dtype=torch.float8_e4m3fn)  # noqa: E731
+    args = [f8(2, 128), torch.ones(2, 1), f8(3, 128), torch.ones(1, 1), torch.zeros(3)]
+    args[which].requires_grad_()
+    with pytest.raises(RuntimeError, match="has no gradient"):
+        ot.project_joiner_fp8(*args)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="one HIP device"):
+        ot.project_joiner_fp8(*args)
