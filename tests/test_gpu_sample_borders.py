@@ -245,3 +245,38 @@ def test_top_p_where_sums_of_32_bits_are_far_off(make, V, top_p, device):
     assert s.tolist() == want
     want_lp = z[want] - math.log(run[-1])
     assert (np.abs(lp.double().cpu().numpy() - want_lp) <= 2.0 ** -24 * np.abs(want_lp) + 2.0 ** -30).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [16385, 50000, 131072])
+def test_slices_with_settings_of_each_row(V, dtype, device):
+    """Rows in slices, each with a temperature, top_p and min_p of its own: greedy rows, rows without
+    cuts, rows of every one of them, rows without an answer."""
+    rng = np.random.default_rng(V)
+    rows = 40
+    x = (rng.standard_normal((rows, V)) * 2).astype(np.float32)
+    x[::7, 0] += 12.0  # nearly all of a row in one entry
+    x[5] = -np.inf
+    x[9, V - 2] = np.nan
+    t = torch.from_numpy(x).to(device).to(DT[dtype])
+    x = t.float().cpu().numpy()
+    u = rng.random(rows).astype(np.float32)
+    u[12] = np.nan
+    T = rng.choice([0.0, 0.4, 1.0, 1.7, -1.0, math.nan], rows).astype(np.float32)
+    p = rng.choice([0.0, 0.3, 0.9, 0.999, 1.0, 4.0, math.nan], rows).astype(np.float32)
+    q = rng.choice([0.0, 1e-3, 0.2, 1.0, math.nan], rows).astype(np.float32)
+    dev = lambda a: torch.from_numpy(a).to(device)  # noqa: E731
+    s, lp = ot.sample_symbols(t, dev(u), temperature=dev(T), top_p=dev(p), min_p=dev(q))
+    want, want_lp = ao.sample(x, u, T, 0, np.where(np.isnan(p), 1.0, p), np.where(np.isnan(q), 0.0, q))
+    assert np.array_equal(s.cpu().numpy(), want)
+    lp = lp.double().cpu().numpy()
+    fine = np.isfinite(want_lp)
+    assert np.array_equal(lp[~fine], want_lp[~fine])
+    assert (np.abs(lp - want_lp)[fine] <= 2.0 ** -24 * np.abs(want_lp[fine]) + 2.0 ** -35).all()
+    for settings in (dict(temperature=dev(T), top_p=0.9), dict(top_p=dev(p)), dict(temperature=0.8, min_p=dev(q)),
+                     dict(temperature=dev(T), top_p=0.5, min_p=dev(q))):
+        host = {"temperature": 1.0, "top_p": 1.0, "min_p": 0.0}
+        host.update({k: v.cpu().numpy() if torch.is_tensor(v) else v for k, v in settings.items()})
+        host = {k: np.where(np.isnan(v), {"temperature": 0.0, "top_p": 1.0, "min_p": 0.0}[k], v) for k, v in host.items()}
+        s, _ = ot.sample_symbols(t, dev(u), **settings)
+        assert np.array_equal(s.cpu().numpy(), ao.sample(x, u, top_k=0, **host)[0]), list(settings)
