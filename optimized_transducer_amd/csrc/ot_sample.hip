@@ -336,14 +336,14 @@ struct Drawn {
   float log_prob;
 };
 
-// (x - m) / T - log(total) in 64 bits, rounded once; total >= 1.  log(total) = a + 2 artanh((total - e) /
-// (total + e)) with a = log of e = 2^b, b the hardware's logarithm of 32 bits: artanh's first term is
-// enough (its argument is below 2^-20, the next term below 2^-60), and the polynomial of the weights
-// serves again (the library's logarithm keeps 12 more registers of constants over a kernel's loop:
-// 751 992 x 500 float32 519 us and 504 so, 4096 x 16 000 with top_p 712 and 629)
-__device__ __forceinline__ float log_probability(float logit, float m, float T, double total) {
-  const double b = __builtin_amdgcn_logf((float)total), e = power_of_2(b);
-  return (float)(((double)logit - m) / T - (b * 0.69314718055994531 + 2.0 * ((total - e) / (total + e))));
+// (x - m) / T - log(total) in 64 bits, rounded once; c = log2(e) / T, total >= 1.  With b the hardware's
+// log2 of 32 bits, total * 2^-b = 1 + q and log(total) = b ln 2 + q - q^2 / 2: |q| < 2^-18, and what is left
+// out is below 2^-55.  The polynomial of the weights serves again (the library's logarithm keeps 12 more
+// registers of constants over a kernel's loop: 751 992 x 500 float32 519 us and 504 so, 4096 x 16 000 with
+// top_p 712 and 629)
+__device__ __forceinline__ float log_probability(float logit, float m, double c, double total) {
+  const double b = __builtin_amdgcn_logf((float)total), q = __builtin_fma(total, power_of_2(-b), -1.0);
+  return (float)((((double)logit - m) * c - b) * 0.69314718055994531 - (q - 0.5 * q * q));
 }
 
 // Draws from a row with a finite largest entry m at a temperature above 0.  Every thread of the
@@ -360,7 +360,7 @@ struct Sampler {
   const RowGroup<WAVES> &g;
   const void *row;
   const int V, per_wave;
-  const float m, T_;
+  const float m;
   const Weight weight;
   float (&x)[kHeld ? CHUNKS : 1][VEC];
   double w[kHeldWeights ? CHUNKS : 1][VEC];
@@ -376,7 +376,7 @@ struct Sampler {
 
   __device__ __forceinline__ Sampler(const RowGroup<WAVES> &g_, const void *row_, int V_, int per_wave_, float m_,
                                      float temperature, float (&x_)[kHeld ? CHUNKS : 1][VEC])
-      : g(g_), row(row_), V(V_), per_wave(per_wave_), m(m_), T_(temperature), weight(m_, temperature), x(x_) {}
+      : g(g_), row(row_), V(V_), per_wave(per_wave_), m(m_), weight(m_, temperature), x(x_) {}
 
   __device__ __forceinline__ int chunks() const { return kHeld ? CHUNKS : per_wave; }
   __device__ __forceinline__ int first_index(int j) const {
@@ -971,7 +971,7 @@ struct Sampler {
       float logit;
       double total;
       draw_alone(u, symbol, logit, total);
-      return {symbol, log_probability(logit, m, T_, total)};
+      return {symbol, log_probability(logit, m, weight.c, total)};
     } else {
       // totals of the waves' parts, then the part, the chunk, the lane and the element in which
       // the running sum passes u * total
@@ -1043,7 +1043,7 @@ struct Sampler {
         for (int k = 0; k < WAVES; ++k) symbol = max(symbol, g.s.count[k]);
         logit = load_element<T>(row, symbol);
       }
-      return {symbol, log_probability(logit, m, T_, total)};
+      return {symbol, log_probability(logit, m, weight.c, total)};
     }
   }
 };
@@ -1338,7 +1338,7 @@ __global__ __launch_bounds__(kBlock, 4) void sample_plain_kernel(const void *__r
     if (g.lane < n) {
       symbols[row0 + g.lane] = my_symbol;
       log_probs[row0 + g.lane] = my_symbol < 0 ? OT_NEG_INF
-                                 : my_T > 0.f  ? log_probability(my_logit, my_m, my_T, my_total)
+                                 : my_T > 0.f  ? log_probability(my_logit, my_m, Weight(my_m, my_T).c, my_total)
                                                : 0.f;
     }
   }
@@ -1802,13 +1802,14 @@ static int launch_slices(const void *logits, int64_t row_stride, int64_t rows, i
 }
 
 // Waves per SIMD: as many as leave the elements of a thread in registers.
-constexpr int sample_occupancy(int waves, int elements) {
-  return waves == 16 || waves == 1 ? 4 : waves == 4 && elements <= 16 ? 3 : 2;
+constexpr int sample_occupancy(int waves, int elements, bool filter) {
+  return waves == 16 || waves == 1 ? 4 : waves == 4 && (elements <= 16 || !filter) ? 3 : 2;
 }
 
 // ROWS groups of WAVES waves per workgroup, a row each
 template <class T, int WAVES, int ROWS, int CHUNKS, bool FILTER>
-__global__ __launch_bounds__(WAVES * ROWS * kWave, sample_occupancy(WAVES, CHUNKS * kSampleVec<T>)) void sample_kernel(
+__global__ __launch_bounds__(WAVES * ROWS * kWave, sample_occupancy(WAVES, CHUNKS * kSampleVec<T>, FILTER)) void
+sample_kernel(
     const void *__restrict__ logits, int64_t row_stride, int64_t rows, int V, const float *__restrict__ uniform,
     SampleSettings set, int32_t *__restrict__ symbols, float *__restrict__ log_probs) {
   static_assert(ROWS == 1 || WAVES == 1, "barriers are per workgroup");
