@@ -489,7 +489,9 @@ int ot_quantize_blocks(const void *x, int32_t dtype, int64_t row_stride,
  * multiple of 16; x_scale (rows, ceil(D / 128)), weight_scale (ceil(V / 128),
  * ceil(D / 128)), bias (V) or NULL, float32.  With den the caller lends
  * ot_joiner_project_blocks_workspace_bytes(rows, V) bytes, 8-byte aligned,
- * contents irrelevant before and after.  rows = 0 does nothing. */
+ * contents irrelevant before and after: enough for a partial result of each 64
+ * entries and row, whatever D (long batches write fewer of them, or none).
+ * rows = 0 does nothing. */
 size_t ot_joiner_project_blocks_workspace_bytes(int64_t rows, int32_t V);
 int ot_joiner_project_blocks(const void *x, const float *x_scale,
                              const void *weight, const float *weight_scale,
@@ -513,7 +515,10 @@ int ot_joiner_project_blocks(const void *x, const float *x_scale,
  *     log_probs[r] = log(w_symbol / total)
  * T <= 0 or NaN: the first of the largest entries, log_probs 0.  A row without
  * a largest finite entry (all -inf, a NaN, +inf) or with uniform NaN gives
- * symbol -1 and log_probs -inf.  Weights and sums behave as in 64 bits.
+ * symbol -1 and log_probs -inf.  Weights and sums behave as in 64 bits: a weight
+ * is within (|(x_i - m) / T| + 1) * 2^-51 of itself, and where a border lies
+ * within a rounding of the sums the answer is an entry at that border, never an
+ * excluded one.  log_probs are rounded once.
  *
  * logits (rows, V) of `dtype` (any of the three), element (r, v) at
  * logits[r * row_stride + v]; uniform, symbols, log_probs (rows).  Each setting

@@ -86,22 +86,24 @@ def sample_symbols(logits: torch.Tensor, uniform: torch.Tensor,
     w_i >= ``min_p``.  The symbol is the first index, in index order, whose running sum of
     remaining weights exceeds ``uniform`` times their total.  Weights and sums behave as in
     64 bits: only where a border lies within a rounding of those can the symbol depend on how
-    many rows are drawn from at once.
+    many rows are drawn from at once, and it is then one of the entries at that border.
 
     Args:
       logits: (rows, V) float32, float16 or bfloat16 on a HIP device; any row pitch (columns
         ``[:V]`` of padded logits, say); masked entries are -inf; rows may be 0.
-      uniform: (rows,) float32 numbers of [0, 1), e.g. ``torch.rand(rows, device=...)``.
+      uniform: (rows,) float32 numbers of [0, 1), e.g. ``torch.rand(rows, device=...)``; small ones
+        count as they are, whatever the entries in front of which they fall.
       temperature: >= 0; 0 takes the first of the largest entries.
       top_k: >= 0; 0 leaves it out.
       top_p: [0, 1]; 1 leaves it out.
       min_p: [0, 1]; 0 leaves it out.
-        Each setting is one number or a tensor of shape (rows,) (float32; ``top_k`` int32).
+        Each setting is one number or a tensor of shape (rows,) (float32; ``top_k`` int32); numbers are
+        taken as float32 too, so that a temperature below its smallest value is 0.
         Numbers out of range are refused; in a tensor a temperature that is not positive
         counts as 0, top_k < 0 as 0, top_p as clamped to [0, 1] and min_p too.
     Returns:
       (symbols, log_probs): (rows,) int32 and (rows,) float32 = log(w_symbol / total) under
-      the distribution drawn from (0 at temperature 0), without a gradient.  A row without a
+      the distribution drawn from (0 at temperature 0), rounded once, without a gradient.  A row without a
       largest finite entry (all -inf, a NaN, +inf), or whose number is NaN, gives -1 and -inf.
     """
     t, t_value = _setting(temperature)

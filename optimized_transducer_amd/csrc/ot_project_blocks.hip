@@ -172,10 +172,13 @@ __global__ __launch_bounds__(kBlock) void project_blocks_small_kernel(
 //   ALIGNED: 16 bytes of logits start at a multiple of 4 bytes.  Else (2-byte logits of an odd V)
 //   they go through ordinary stores, which any element may start at, and not the buffer view's:
 //   100 000 x 512 x 501 float16 146 us with stores of single elements, 93 so
-// What bounds it: the stores of the logits, in partial lines where V * the size of a logit is no
-// multiple of 128 bytes, and behind them the matrix instructions.  751 992 x 512 x 500 bfloat16 with
-// denominators 0.53 ms, 725 TFLOP/s and 2.2 TB/s; 149 346 x 512 x 5000 float32 1.24 ms, 619 TFLOP/s
-// and 2.5 TB/s (tiles straight from memory, as the small kernel's: 3.19 and 6.26 ms).
+// What bounds it: vector instructions (7.3 for each matrix instruction: widening, scales, rounding,
+// exponentials) and matrix instructions follow each other, with two waves a SIMD to overlap them.  751 992 x
+// 512 x 500 bfloat16 with denominators: vector 64 % and matrix instructions 33 % of the cycles, 0.54 ms, 711
+// TFLOP/s and 2.2 TB/s (where it takes 0.55, 0.52 without the stores, 0.37 without the matrix instructions,
+// 0.49 without denominators).  149 346 x 512 x 5000 float32: 46 % and 27 %, and the stores, 1.24 ms, 617
+// TFLOP/s and 2.5 TB/s (0.99 without the stores, 1.17 without the matrix instructions).  Tiles straight from memory, as the
+// small kernel's, take 3.19 and 6.26 ms.
 // Lane l holds bytes [64 q + 16 (l / 16), + 16) of a block of row l % 16 (q = 0, 1); the first 8
 // feed matrix instruction 2 q and the others 2 q + 1, in both operands alike.
 template <class T, int KB, bool ALIGNED, bool DEN>
@@ -750,6 +753,9 @@ static int launch_project_blocks(const unsigned char *x, const float *xs, const 
   if (!few && V < (1 << 21) && D < (1 << 24)) {
 #define OT_PROJECT_WIDE(KB_) \
   return launch_project_blocks_wide<T, KB_>(x, xs, w, ws, bias, rows, D, V, logits, den, parts, cus, s)
+    // us by the wide kernel and by the deep one: 1024 x 512 x 500 bfloat16 11.6 and 11.3, 8000 x 512 x 500
+    // 18 and 15, 100 000 x 512 x 500 83 and 99, 751 992 x 512 x 500 511 and 723, 751 992 x 128 x 500 324 and
+    // 457; float32 2000 x 512 x 5000 27 and 30, 100 000 x 384 x 1001 184 and 201
     if (nblocks == 1) OT_PROJECT_WIDE(1);
     if (nblocks == 2) OT_PROJECT_WIDE(2);
     if (nblocks == 3) OT_PROJECT_WIDE(3);

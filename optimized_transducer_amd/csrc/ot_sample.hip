@@ -16,7 +16,8 @@
 // and sums are 64-bit.  This chip's vector units do 64-bit multiply-adds at the rate of
 // (unpacked) 32-bit ones, so a weight costs 19 such instructions (a range reduction and a
 // polynomial for 2^f) where a 32-bit one through the hardware's 2^x costs 8 and the transcendental
-// unit.
+// unit.  A sum over lanes is never recovered from a difference, and a lane without a weight is never
+// drawn from: its sum may be a rounding larger than its neighbour's.
 //
 // How the cuts are found: a wave that holds its row sorts it and reads both of them off the order
 // (32 x 512 float32, settings per row, 6.3 us, 11.7 by histograms).  Longer rows are not sorted: a
@@ -26,8 +27,9 @@
 //
 // Who works on a row (what bounds it; times at T = 1 and sigma 2):
 //   a wave                short rows, up to 512 (float32) or 1024 elements, in registers, and no
-//                         barrier.  Without cuts a wave takes a batch of them: the 64-bit weights
-//                         bound it (751 992 x 500 float32 0.49 ms, 3.1 TB/s)
+//                         barrier.  Without cuts a wave takes a batch of them: vector instructions
+//                         bound it, 44 per weight, 91 % of the cycles (751 992 x 500 float32 0.51 ms,
+//                         2.9 TB/s)
 //   4, 8 or 16 waves      rows up to 16384, in registers; of all the waves only the wide steps
 //                         profit, so that the barriers and scans of the cuts bound it.  A top_k of
 //                         512 at most is found by all of them, and one wave goes on with what is left
@@ -55,7 +57,10 @@ struct SampleSettings {
 };
 
 constexpr int kSampleBins = 256;
-constexpr int kSampleFew = 512;  // entries that one wave takes over from the others
+// Entries that one wave takes over from the others.  us with 256, 512 and 1024: 4096 x 5000 float16 with
+// top_k 200 and the other cuts 80, 85, 97, top_k 250 97, 86, 97, top_k 400 182, 86, 98, top_k 700 187, 188,
+// 99; 64 x 2000 float32 with top_k 50 7.6, 8.6, 11.2
+constexpr int kSampleFew = 512;
 constexpr float kInf = __builtin_huge_valf();
 
 // ---- wave-wide helpers ----------------------------------------------------------------------
@@ -1850,7 +1855,9 @@ static int launch_sample_kernel(const void *logits, int64_t row_stride, int64_t 
 template <class T, int CHUNKS>
 static int launch_sample_plain(const void *logits, int64_t row_stride, int64_t rows, int32_t V, const float *uniform,
                                const SampleSettings &set, int32_t *symbols, float *log_probs, hipStream_t s) {
-  // 7 waves per SIMD of 256 compute units are resident; 16 rows a batch fill a line of answers
+  // 7 waves per SIMD of 256 compute units are resident; 16 rows a batch fill a line of answers.  us with
+  // batches of 1, 4, 16 and 64 rows: 30 000 x 500 float32 29, 25, 24, 24, 751 992 x 500 633, 532, 503, 480,
+  // 751 992 x 100 436, 352, 325, 302
   constexpr int64_t kWaves = 256 * 4 * 7;
   const int batch = (int)(rows <= kWaves ? 1 : rows >= 16 * kWaves ? 16 : (rows + kWaves - 1) / kWaves);
   const int64_t per_group = (int64_t)kWavesPerBlock * batch, groups = (rows + per_group - 1) / per_group;
@@ -1872,7 +1879,10 @@ static int launch_sample(const void *logits, int64_t row_stride, int64_t rows, i
                                                        log_probs, s)
   if constexpr (FILTER) {
     if (V > 2 * kChunk && !set.top_k && set.top_k_value > 0 && set.top_k_value <= kSampleFew) {
-      // a batch of rows per workgroup where there are rows for all compute units
+      // A batch of four rows per workgroup, a wave each for the few, where there are rows for all compute
+      // units; us by one row and by four: 1024 x 2000 float32 14, 22, 2048 x 2000 26, 25, 4096 x 2000 49,
+      // 36, 20 011 x 5000 float16 893, 404 (1024 x 5000 float16 47, 37 and 512 x 5000 25, 36: the border
+      // is right for the shorter of them).  Longer rows take 8 or 16 waves, and one row at a time.
       if (rows >= 2048) {
         if (V <= 2048) OT_SAMPLE_FEW(4, 2048 / 4 / kChunk, 4);
         if (V <= 4096) OT_SAMPLE_FEW(4, 4096 / 4 / kChunk, 4);
@@ -1895,6 +1905,8 @@ static int launch_sample(const void *logits, int64_t row_stride, int64_t rows, i
     if (V <= 2 * kChunk)
       return launch_sample_plain<T, 2>(logits, row_stride, rows, V, uniform, set, symbols, log_probs, s);
   }
+  // (4 waves up to 6144 entries; 8 waves from 4097 on take 20 000 x 5000 float32 244 us without cuts and
+  // 1172 with top_p, 4 waves 178 and 718; 64 x 5000 8 and 17 both)
   if (V <= 2048) OT_SAMPLE(4, 1, 2048 / 4 / kChunk);
   if (V <= 4096) OT_SAMPLE(4, 1, 4096 / 4 / kChunk);
   if (V <= 6144) OT_SAMPLE(4, 1, 6144 / 4 / kChunk);
