@@ -810,7 +810,8 @@ struct Sampler {
     // Where the entries above v reach `want` already, or those at it do not, v is somewhere else: next
     // to it for a few steps, and then by halving what is left of the values' keys (32-bit sums of many
     // weights in one bin can be off by thousands of entries, and stop growing at 2^24 times a weight).
-    unsigned below = order_key(lowest) - 1, beyond = order_key(m) + 1;  // v's key is between them
+    // (keys, and not their values, which both zeros have in common: every answer takes its key out)
+    unsigned key = order_key(v), below = order_key(lowest) - 1, beyond = order_key(m) + 1;
     int at_v, went = 0;
     double wv;
     bool last = false;
@@ -819,12 +820,13 @@ struct Sampler {
       wv = weight(v);
       const int go = sum >= want && v < m ? 1 : sum + at_v * wv < want && v > lowest ? -1 : 0;
       if (last || go == 0 || go == -went) break;  // (back and forth: the border lies within a rounding)
-      if (go > 0) below = order_key(v);
-      else beyond = order_key(v);
+      if (go > 0) below = key;
+      else beyond = key;
       went = step < kNearSteps ? go : 0;
       last = step >= kNearSteps && beyond - below <= 1;  // nothing left: a rounding again
       if (step >= kNearSteps && !last) {
-        v = key_value(below + (beyond - below) / 2);  // (`go` is not 0 where no entry is)
+        key = below + (beyond - below) / 2;
+        v = key_value(key);  // (`go` is not 0 where no entry is)
         continue;
       }
       if (last) v = key_value(below);
@@ -838,6 +840,7 @@ struct Sampler {
       });
       g.extremes(down, up);
       v = last || go > 0 ? up : down;
+      key = order_key(v);
     }
     // of the entries at v, number j (from 0) remains if sum + j * wv < want
     int n = at_v;

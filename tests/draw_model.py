@@ -57,3 +57,43 @@ def draw(w, u):
                     break
         out[r] = lane * w.shape[2] + at
     return out
+
+
+def order_key(x):
+    """Unsigned integers that order like float32 values, both zeros alike."""
+    b = int(np.array([np.float32(x) + np.float32(0.0)], np.float32).view(np.uint32)[0])
+    return b ^ (0xFFFFFFFF if b >> 31 else 0x80000000)
+
+
+def key_value(key):
+    b = key ^ (0x80000000 if key >> 31 else 0xFFFFFFFF)
+    return float(np.array([b], np.uint32).view(np.float32)[0])
+
+
+def search(values, v, answer, near=4):
+    """The values that the search for top_p's cut looks at, starting from v: values is the row's,
+    answer(v) 1, -1 or 0 for a cut above, below or at v."""
+    values = sorted(set(values))
+    lowest, largest = values[0], values[-1]
+    below, beyond = order_key(lowest) - 1, order_key(largest) + 1
+    key, went, last, seen, step = order_key(v), 0, False, [], 0
+    while True:
+        seen.append(v)
+        go = answer(v)
+        if last or go == 0 or go == -went:
+            return seen
+        if go > 0:
+            below = key
+        else:
+            beyond = key
+        went = go if step < near else 0
+        last = step >= near and beyond - below <= 1
+        if step >= near and not last:
+            key = below + (beyond - below) // 2
+            v = key_value(key)
+        else:
+            if last:
+                v = key_value(below)
+            v = min(y for y in values if y > v) if last or go > 0 else max(y for y in values if y < v)
+            key = order_key(v)
+        step += 1

@@ -67,3 +67,26 @@ def test_draw_of_small_numbers(vec):
         middle = (run + np.concatenate([[0.0], run[:-1]])) / 2 / run[-1]
         got = draw_model.draw(np.repeat(w, len(at), 0), middle)
         assert np.array_equal(got, at)
+
+
+def test_search_for_the_cut_ends_at_it():
+    rng = np.random.default_rng(5)
+    values = [float(v) for v in (rng.standard_normal(400) * 3).astype(np.float32)] + [0.0, 1e-45, -1e-45]
+    for cut in values[::7] + [0.0, 1e-45, -1e-45]:
+        for start in (min(values), 0.0, max(values), values[17]):
+            answer = lambda v: 0 if v == cut else 1 if v < cut else -1  # noqa: E731
+            seen = draw_model.search(values, start, answer)
+            assert seen[-1] == cut and len(seen) <= 40
+
+
+@pytest.mark.parametrize("turn", [0.0, -1e-45, 1e-45, 0.3])
+@pytest.mark.parametrize("far", [-5.0, 5.0])
+def test_search_for_the_cut_ends_where_sums_contradict_each_other(turn, far):
+    """Roundings can put the cut above one value and below the next, and at neither: the search ends
+    there all the same, at a value of the row, around zero too, whose two signs are one value."""
+    values = [float(v) for v in np.linspace(-6, 6, 200).astype(np.float32)] + [0.0, 1e-45, -1e-45]
+    start = min(values) if far < 0 else max(values)
+    for at_turn in (1, -1):
+        answer = lambda v: 1 if v < turn else -1 if v > turn else at_turn  # noqa: E731
+        seen = draw_model.search(values, start, answer)
+        assert len(seen) <= 40 and seen[-1] in values
