@@ -177,8 +177,8 @@ __global__ __launch_bounds__(kBlock) void project_blocks_small_kernel(
 // 512 x 500 bfloat16 with denominators: vector 64 % and matrix instructions 33 % of the cycles, 0.54 ms, 711
 // TFLOP/s and 2.2 TB/s (where it takes 0.55, 0.52 without the stores, 0.37 without the matrix instructions,
 // 0.49 without denominators).  149 346 x 512 x 5000 float32: 46 % and 27 %, and the stores, 1.24 ms, 617
-// TFLOP/s and 2.5 TB/s (0.99 without the stores, 1.17 without the matrix instructions).  Tiles straight from memory, as the
-// small kernel's, take 3.19 and 6.26 ms.
+// TFLOP/s and 2.5 TB/s (0.99 without the stores, 1.17 without the matrix instructions).  Tiles straight
+// from memory, as the small kernel's, take 3.19 and 6.26 ms.
 // Lane l holds bytes [64 q + 16 (l / 16), + 16) of a block of row l % 16 (q = 0, 1); the first 8
 // feed matrix instruction 2 q and the others 2 q + 1, in both operands alike.
 template <class T, int KB, bool ALIGNED, bool DEN>
